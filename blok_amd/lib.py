@@ -85,6 +85,24 @@ class KxExpertsConfig(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("width", "ff", "experts", "top", "cols")] + [(n, C.c_float) for n in ("limit", "alpha", "bias")]
 
 
+class KxPagedConfig(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("heads", "kv_heads", "dim", "vdim", "page", "block", "rot", "pairs", "size")] + [
+        ("scale", C.c_float), ("base", C.c_double)]
+
+
+class KxPagedCache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("d_k", "d_v", "d_k_scale", "d_v_scale", "d_table")] + [("pages", C.c_int32), ("table_ld", C.c_int32)]
+
+
+class KxPagedRows(C.Structure):
+    _fields_ = [("d_start", C.c_void_p), ("d_pos", C.c_void_p)] + [(n, C.c_int32) for n in ("batch", "tokens", "longest")]
+
+
+class KxFp8Args(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("x_f32", "out_f32", "tokens", "rows", "cols", "ld", "x_ld", "out_ld")] + [
+        (n, C.c_void_p) for n in ("d_w", "d_w_scale", "d_x", "d_out")]
+
+
 DTYPES = {"bfloat16": 0, "float32": 1}
 
 _P, _I, _U64, _F, _SZ = C.c_void_p, C.c_int32, C.c_uint64, C.c_float, C.c_size_t
@@ -176,6 +194,15 @@ _SIGS = {
     "kx_experts_destroy": [_P],
     "kx_experts_run": [_P, _P, _P, _F, _P, _P, _P, _P, _P, _P, _I, _P, _P],
     "kx_linear_run": [C.POINTER(KxLinearArgs), _P, _P],
+    "kx_paged_create": [C.POINTER(KxPagedConfig), _P, C.c_int, _I, _I, _PP],
+    "kx_paged_destroy": [_P],
+    "kx_paged_append": [_P, C.POINTER(KxPagedCache), C.POINTER(KxPagedRows), _P, _I, _I, _I, _P],
+    "kx_paged_attend": [_P, C.POINTER(KxPagedCache), C.POINTER(KxPagedRows), _P, _I, _I, _P, _I, _P],
+    "kx_paged_read": [_P, C.POINTER(KxPagedCache), C.POINTER(KxPagedRows), _P, _I, _P, _I, _P],
+    "kx_paged_faults": [_P, C.POINTER(C.c_int32), _P],
+    "kx_fp8_create": [_I, _I, _PP],
+    "kx_fp8_destroy": [_P],
+    "kx_fp8_run": [_P, C.POINTER(KxFp8Args), _P],
     "kx_open_options_default": [C.POINTER(KxOpenOptions)],
     "kx_model_open": [C.c_char_p, C.POINTER(KxOpenOptions), _PP],
     "kx_model_probe": [C.c_char_p, C.POINTER(KxModelShape)],

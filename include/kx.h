@@ -380,6 +380,79 @@ typedef struct kx_linear_args {
   void *d_prev_out, *d_mid;
 } kx_linear_args;
 int kx_linear_run(const kx_linear_args *args, void *d_row_scratch, void *stream); /* scratch: tokens * ld elements of the format per variant of the rows */
+/* ---- a paged cache in 8 bits -----------------------------------------------------------------
+ * Keys and values of sequences of different lengths, appended and attended to in one call for a whole batch.  No counterparts in the
+ * reference.  The cache is the caller's memory: a page holds `page` positions (a multiple of 64) of all heads of keys, and d_table
+ * i32 [batch][table_ld] says which page has positions page i .. page (i + 1) - 1 of a sequence.
+ *   d_k [pages][kv_heads][page][dp], d_v [pages][kv_heads][page / 64][vp][64]: e4m3 codes; dp and vp are the widths of the smallest of
+ *   64 | 64, 128 | 128, 192 | 128 and 256 | 256 that hold dim and vdim, zero beyond these.  Token t of 64 is at place
+ *   (t / 4 % 4) 16 + t / 32 8 + t / 16 % 2 4 + t % 4 of a row of d_v.
+ *   d_k_scale, d_v_scale f32 [pages][kv_heads][page / block]: an element is its code times the scale of its block of 16, 32 or 64 positions,
+ *   2^e with the least e >= -100 that keeps the block's largest finite magnitude within 448 * 2^e.
+ * Nothing has to be initialised, and d_k and d_v begin at multiples of 16 bytes.  The rows of a call are those of a ragged batch: sequence b has rows d_start[b] .. d_start[b + 1] - 1 (d_start i32 [batch + 1]), at
+ * positions from d_pos[b] on (i32 [batch]); a sequence may have none.  `tokens`: rows that there is memory for; rows behind d_start[batch]
+ * are not read or written.  `longest`: positions of the longest sequence, the new ones among them, by which the work is shared out; a longer one costs time
+ * and nothing else.  Tables lie on the device, so that a captured call replays with other lengths and pages.
+ * kx_paged_create: handle with scratch for calls of up to max_batch sequences and, appending and attending, max_tokens rows, on the current device.  Queries and keys
+ *   are turned by their positions: the first `rot` dimensions in pairs (d, d + rot / 2), with pairs = 1 (2 d, 2 d + 1), by position * h_freq[d]
+ *   (rot / 2 doubles), or base^(-2 d / rot) where h_freq is NULL.  f32: results are float, and as exact; 0: bf16.  Calls on
+ *   one handle that overlap (two streams, two threads, two graphs) race; calls one after another do not.  One handle serves any number of caches.
+ * kx_paged_append: d_proj f32 [tokens][proj_ld] holds the rows' keys [kv_heads][dim] from column k_off on and values [kv_heads][vdim] from
+ *   v_off on.  A block that the new rows begin takes its scale from them; one that has older tokens keeps its scale or, if they need a
+ *   larger one, has its older codes divided by what it grew.  Positions behind the last appended one hold nothing from then on.  What is not finite
+ *   is NaN in the cache.  Two sequences of a call must not append to the same page.
+ * kx_paged_attend: out = softmax(scale q k^T) v over the positions up to a row's own, the last `size` of them where size > 0; queries [heads][dim] of
+ *   d_proj from q_off on, d_out [tokens][out_ld] of heads * vdim.  Head h reads head h / (heads / kv_heads) of keys.  The rows' own keys and
+ *   values have been appended before.
+ * kx_paged_read: the keys and values that the cache has at the rows' positions, bf16 [tokens][k_ld] and [tokens][v_ld].
+ * kx_paged_faults: whether the tables of earlier calls held a page outside [0, pages) (KX_PAGED_BAD_PAGE: appended rows are dropped, its positions are not
+ *   seen), positions outside the table (_BAD_POSITION) or rows outside [0, tokens] (_BAD_ROWS; such sequences are left out).  Synchronises, and clears them.  A result that
+ *   no position was left for is 0. */
+#define KX_PAGED_BAD_PAGE 1
+#define KX_PAGED_BAD_POSITION 2
+#define KX_PAGED_BAD_ROWS 4
+typedef struct kx_paged_config {
+  int32_t heads, kv_heads, dim, vdim, page, block, rot, pairs, size;
+  float scale;
+  double base;
+} kx_paged_config;
+typedef struct kx_paged_cache {
+  void *d_k, *d_v;
+  float *d_k_scale, *d_v_scale;
+  const int32_t *d_table;
+  int32_t pages, table_ld;
+} kx_paged_cache;
+typedef struct kx_paged_rows {
+  const int32_t *d_start, *d_pos;
+  int32_t batch, tokens, longest;
+} kx_paged_rows;
+typedef struct kx_paged kx_paged;
+int kx_paged_create(const kx_paged_config *cfg, const double *h_freq, int f32, int32_t max_batch, int32_t max_tokens, kx_paged **out);
+int kx_paged_destroy(kx_paged *p);
+int kx_paged_append(kx_paged *p, const kx_paged_cache *cache, const kx_paged_rows *rows, const void *d_proj, int32_t proj_ld, int32_t k_off,
+                    int32_t v_off, void *stream);
+int kx_paged_attend(kx_paged *p, const kx_paged_cache *cache, const kx_paged_rows *rows, const void *d_proj, int32_t proj_ld, int32_t q_off,
+                    void *d_out, int32_t out_ld, void *stream);
+int kx_paged_read(kx_paged *p, const kx_paged_cache *cache, const kx_paged_rows *rows, void *d_k, int32_t k_ld, void *d_v, int32_t v_ld, void *stream);
+int kx_paged_faults(kx_paged *p, int32_t *h_bits, void *stream);
+/* ---- products with 8-bit matrices ----------------------------------------------------------
+ * kx_fp8_run: y = W x for matrices of e4m3 elements with a scale for each block of 128 x 128, as block-scaled checkpoints have them: d_w [rows][ld], ld a
+ * multiple of 128, zero beyond cols; d_w_scale f32 [ceil(rows / 128)][ceil(cols / 128)]; element = code * scale.  A row of x (d_x [tokens][x_ld], float or
+ * bf16) is rounded to e4m3 with a scale 2^e for each 128 columns, the least e >= -100 that keeps their largest finite magnitude within
+ * 448 * 2^e; what is not finite becomes NaN.  Products and sums are 32-bit; d_out [tokens][out_ld] is float or bf16.  d_w begins at a multiple of 16
+ * bytes.  No counterpart in the reference.  kx_fp8_create: scratch for rows of up to max_cols columns, max_tokens of them, on the current device;
+ * calls on one handle that overlap race. */
+typedef struct kx_fp8_args {
+  int32_t x_f32, out_f32, tokens, rows, cols, ld, x_ld, out_ld;
+  const void *d_w;
+  const float *d_w_scale;
+  const void *d_x;
+  void *d_out;
+} kx_fp8_args;
+typedef struct kx_fp8 kx_fp8;
+int kx_fp8_create(int32_t max_tokens, int32_t max_cols, kx_fp8 **out);
+int kx_fp8_destroy(kx_fp8 *p);
+int kx_fp8_run(kx_fp8 *p, const kx_fp8_args *args, void *stream);
 /* ---- model directories ---------------------------------------------------------------------
  * kx_model_open  : reads <dir>/config.json, finds the design it names in the library's registry and opens the model
  *                  with it.  Three designs are known: Kimi-K2 (config.json of the checkpoint with runtime-index.blok
