@@ -17,6 +17,12 @@ struct KxFp8Args {
   bool x_f32 = false, out_f32 = false;
   int blocks = 0;                   // of 128 columns
   uint8_t *xc = nullptr;            // scratch: codes [tokens][blocks * 128]
-  uint8_t *xe = nullptr;            // scratch: e + 127, [tokens][blocks rounded up to 4]
+  uint8_t *xe = nullptr;            // scratch: e + 127, [blocks][groups of 64 tokens][64] (kxfp8::exponent_at)
+  int groups = 0;                   // of 64 tokens, a multiple of 4
+  float *part = nullptr;            // scratch: sums of parts, and who has handed his in
+  size_t part_floats = 0;
+  int *arrived = nullptr;
+  int arrivals = 0;
+  bool pairs = false;               // two neighbouring bf16 results can be stored together
 };
 int kx_fp8_launch(const KxFp8Args &a, hipStream_t st);
