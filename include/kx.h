@@ -440,7 +440,7 @@ int kx_paged_faults(kx_paged *p, int32_t *h_bits, void *stream);
  * multiple of 128, zero beyond cols; d_w_scale f32 [ceil(rows / 128)][ceil(cols / 128)]; element = code * scale.  A row of x (d_x [tokens][x_ld], float or
  * bf16) is rounded to e4m3 with a scale 2^e for each 128 columns, the least e >= -100 that keeps their largest finite magnitude within
  * 448 * 2^e; what is not finite becomes NaN.  Products and sums are 32-bit; d_out [tokens][out_ld] is float or bf16.  d_w begins at a multiple of 16
- * bytes.  No counterpart in the reference.  kx_fp8_create: scratch for rows of up to max_cols columns, max_tokens of them, on the current device;
+ * bytes.  No counterpart in the reference.  kx_fp8_create: scratch for rows of up to max_cols columns (at most 131072), max_tokens of them, on the current device;
  * calls on one handle that overlap race. */
 typedef struct kx_fp8_args {
   int32_t x_f32, out_f32, tokens, rows, cols, ld, x_ld, out_ld;

@@ -56,6 +56,20 @@ def test_large_products(kxlib, tokens, rows, cols, out_f32):
     check(kxlib.kx_fp8_destroy(h))
 
 
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 7, 20, 40, 70])
+def test_long_rows_and_many_rows(kxlib, tokens):
+    """More blocks of columns than lie in LDS at once, shares of rows that begin inside a band of 128, and parts of the columns."""
+    rng = np.random.default_rng(tokens)
+    for rows, cols in ((24, 33000), (130, 9000), (8300, 500), (33000, 130)):
+        say(f"long {tokens} x {rows} x {cols}")
+        c, s, w = S.matrix(rng, rows, cols)
+        h = handle(kxlib, tokens, cols)
+        x = rows_of(rng, tokens, cols, False)
+        for out_f32 in (False, True):
+            near(S.product(kxlib, h, c, s, x, cols, out_f32, False), S.row_codes(x), w, out_f32)
+        check(kxlib.kx_fp8_destroy(h))
+
+
 def test_rows_of_every_size(kxlib):
     """Magnitudes from the smallest to the largest float, blocks of zeros, and what is not finite."""
     rng = np.random.default_rng(9)

@@ -92,7 +92,7 @@ def test_calls_without_a_handle_are_refused():
     assert lib.kx_paged_destroy(None) == 0 and lib.kx_fp8_destroy(None) == 0
     assert lib.kx_fp8_run(None, C.byref(KxFp8Args()), None) != 0
     h = C.c_void_p()
-    for tokens, cols in ((0, 1), (1, 0), (-1, 1), (1, -1), (2 ** 31 - 1, 1), (1, 2 ** 31 - 1)):
+    for tokens, cols in ((0, 1), (1, 0), (-1, 1), (1, -1), (2 ** 31 - 1, 1), (1, 2 ** 17 + 1), (1, 2 ** 31 - 1)):
         assert lib.kx_fp8_create(tokens, cols, C.byref(h)) != 0
     assert lib.kx_fp8_create(1, 1, None) != 0
 
