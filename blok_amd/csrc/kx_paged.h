@@ -9,6 +9,10 @@
 #include <stdint.h>
 #include "kx_paged_place.h"
 
+struct KxDivider {
+  int d = 1;
+  uint32_t m = 0;  // (2^32 - 1) / d
+};
 struct KxPagedSpec {
   int heads = 0, kv_heads = 0, dim = 0, vdim = 0, page = 0, block = 0, rot = 0, pairs = 0, size = 0;
   float scale = 1;
@@ -34,6 +38,8 @@ struct KxPagedArgs {
   size_t part_floats = 0;
   int *arrived = nullptr;
   int arrivals = 0;
+  KxDivider by_g, by_kv, per_page, by_splits;  // heads of a head of keys, heads of keys, groups of a page, parts
+  int block_bits = 0;                          // of the size of a block
   int chunk = 0, splits = 0;     // units of a part (set by the launcher)
 };
 int kx_paged_append_launch(const KxPagedArgs &a, hipStream_t st);
@@ -42,8 +48,18 @@ int kx_paged_attend_launch(bool f32, const KxPagedArgs &a, hipStream_t st);
 // counters and floats of parts that steps of up to max_tokens rows of max_batch sequences can use
 int kx_paged_arrivals(const KxPagedSpec &s, int max_batch, int max_tokens);
 
+namespace kxpage {
+inline KxDivider divider(int d) { return {d, 0xffffffffu / (uint32_t)d}; }
+}
+
 #if defined(__HIPCC__)
 namespace kxpage {
+
+// n / d for n >= 0: 2^32 / d - 1 <= m < 2^32 / d, so that n m / 2^32 lies above n / d - 1 and the whole number below it is the quotient or one less
+__device__ __forceinline__ int quotient(int n, KxDivider v) {
+  const int q = (int)__umulhi((uint32_t)n, v.m);
+  return q + (n - q * v.d >= v.d ? 1 : 0);
+}
 
 // Which sequence a workgroup's task belongs to, where every sequence has count(rows) tasks in a row; n: rows.n is 0 past the last task.  All lanes
 // of a wave call it and get the same.
@@ -61,10 +77,15 @@ __device__ __forceinline__ Task find_task(const KxPagedArgs &a, int task, Count 
     if (r.fault && b0 + lane < a.batch) atomicOr(a.fault, r.fault);
     const int mine = count(r);
     int upto = mine;
+    if (__builtin_amdgcn_ballot_w64(mine > 1)) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(upto, d);
-      if (lane >= d) upto += o;
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+      }
+    } else {  // a step of one row each
+      const uint64_t some = __builtin_amdgcn_ballot_w64(mine > 0);
+      upto += (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
     }
     const uint64_t past = __builtin_amdgcn_ballot_w64(upto > task);
     if (past) {

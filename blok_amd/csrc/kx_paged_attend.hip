@@ -12,10 +12,12 @@
 // Two forms: few columns a sequence (SHARE): the waves of a workgroup take groups of tokens in turn and are added up in LDS; many: every wave has columns
 // of its own.  In both the positions may be split between workgroups, and the last one in adds the parts (kx_arrive.h), in order.
 #include <algorithm>
+#include <type_traits>
 #include "kx_arrive.h"
 #include "kx_common.h"
 #include "kx_math.h"
 #include "kx_paged.h"
+#include "kx_wave.h"
 
 namespace {
 
@@ -23,7 +25,14 @@ using namespace kxpage;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+
+template <class T>
+using Constant = const __attribute__((address_space(4))) T *;  // loaded from by scalar loads, since no launch writes what it reads there
+struct Scales {
+  uint32_t k[4], v[4];
+};
 
 constexpr float NONE = -1e30f;  // M where nothing has been seen
 constexpr int STATS = 4096;     // columns times parts of a task
@@ -36,13 +45,20 @@ __device__ __forceinline__ h8 unpacked(uint32_t lo, uint32_t hi) {
 __device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 // over the four quarters of the wave
 __device__ __forceinline__ float quarters_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  float o = v;
+  kxw::swap_halves32(v, o);
+  v = o = fmaxf(v, o);
+  kxw::swap_rows16(v, o);
+  return fmaxf(v, o);
 }
 __device__ __forceinline__ float quarters_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  float o = v;
+  kxw::swap_halves32(v, o);
+  v = o = v + o;
+  kxw::swap_rows16(v, o);
+  return v + o;
 }
+__device__ __forceinline__ h2 halves_of(float a, float b) { return __builtin_convertvector((f2{a, b}), h2); }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 template <int DP_, int VP_, int NQ_, bool SHARE_, bool F32_>
@@ -53,6 +69,7 @@ struct Form {
   static constexpr size_t PART = (size_t)COLS * (VP + 2);                       // floats of a part: sums, then M and denominator
   static constexpr int REGISTERS = NQ * (DP / 8 * (F32 ? 2 : 1) + VP / 4 + 16) + DP / 4 + VP / 4;
   static constexpr int WAVES = REGISTERS > 200 ? 1 : 2;                         // per SIMD
+  static constexpr int SUB = NQ == 1 ? 4 : 2;                                   // blocks of 16 tokens that are multiplied at a time
   static constexpr int QLD = DP + 4, OLD = 68;                                  // floats of a row in LDS: a query; 64 sums of a column
   static constexpr int Q_FLOATS = (SHARE ? 1 : NW) * 16 * QLD, O_FLOATS = NW * 16 * OLD + 2 * NW * TILE;
   static constexpr int LDS = Q_FLOATS > O_FLOATS ? Q_FLOATS : O_FLOATS;
@@ -65,49 +82,127 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
   __shared__ __attribute__((aligned(16))) float lds[FM::LDS > 2 * STATS ? FM::LDS : 2 * STATS];
   __shared__ int last;
   const KxPagedSpec &s = a.s;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 15, lq = lane >> 4;
-  const int g = s.heads / s.kv_heads, head = blockIdx.x % s.kv_heads, rest = blockIdx.x / s.kv_heads, split = rest % a.splits, task = rest / a.splits;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 15, lq = lane >> 4, g = a.by_g.d;
+  const int rest = quotient(blockIdx.x, a.by_kv), head = blockIdx.x - rest * s.kv_heads, task = quotient(rest, a.by_splits), split = rest - task * a.splits;
   const Task t = find_task(a, task, [&](const Rows &r) { return (r.n * g + COLS - 1) / COLS; });
   if (!t.r.n) return;
   const int R = t.r.n * g, pos = t.r.pos;
+  auto row_of = [&](int column) { return quotient(column, a.by_g); };
   auto low = [&](int hi) { return s.size ? max(hi - s.size + 1, 0) : 0; };
   // the workgroup's units and its part of them
-  const int w0 = t.index * COLS, hi_all = pos + (min(w0 + COLS, R) - 1) / g, first = low(pos + w0 / g) / UNIT, units = hi_all / UNIT - first + 1;
-  const int chunk = max(a.chunk, (units + a.splits - 1) / a.splits), used = (units + chunk - 1) / chunk;
+  const int w0 = t.index * COLS, hi_all = pos + row_of(min(w0 + COLS, R) - 1), first = low(pos + row_of(w0)) / UNIT, units = hi_all / UNIT - first + 1;
+  const int chunk = max(a.chunk, quotient(units + a.splits - 1, a.by_splits)), used = units <= a.chunk ? 1 : (units + chunk - 1) / chunk;
   if (split >= used) return;
   // the wave's columns
   const int c0 = w0 + (SHARE ? 0 : wave * TILE);
   const bool idle = c0 >= R;
-  const int hi_min = pos + min(c0, R - 1) / g, hi_max = pos + min(c0 + TILE - 1, R - 1) / g;
+  const int hi_min = pos + row_of(min(c0, R - 1)), hi_max = pos + row_of(min(c0 + TILE - 1, R - 1));
   int hi[NQ], lo[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    hi[n] = pos + min(c0 + n * 16 + lc, R - 1) / g;
+    hi[n] = pos + row_of(min(c0 + n * 16 + lc, R - 1));
     lo[n] = low(hi[n]);
   }
 
-  // queries: turned by their positions into LDS, 16 columns at a time, and from there to the lanes in the order of the keys' loads
+  // queries: asked for first, a wave a column and a lane a pair of dimensions; turned by their positions into LDS, 16 columns at a time, and from there to the lanes
+  // in the order of the keys' loads
+  constexpr int PP = (DP / 2 + 63) / 64, MINE = SHARE ? 16 / NW : 16;  // pairs of a lane; columns of a wave among 16
+  auto column = [&](int n, int k) { return min(c0 + n * 16 + (SHARE ? k * NW + wave : k), R - 1); };
+  float qx[MINE][PP][2];
+  auto ask_queries = [&](int n) {
+#pragma unroll
+    for (int k = 0; k < MINE; ++k) {
+      const int c = column(n, k), at = row_of(c);
+      const float *const x = a.proj + (size_t)(t.r.first + at) * a.proj_ld + a.q_off + (size_t)(head * g + c - at * g) * s.dim;
+#pragma unroll
+      for (int p = 0; p < PP; ++p) {
+        const int2 d = pair_of(lane + 64 * p, s.rot, s.pairs);
+        qx[k][p][0] = d.x < s.dim ? x[d.x] : 0.0f;
+        qx[k][p][1] = d.y < s.dim ? x[d.y] : 0.0f;
+      }
+    }
+  };
+  double turn[PP];
+#pragma unroll
+  for (int p = 0; p < PP; ++p) turn[p] = lane + 64 * p < s.rot / 2 ? a.turn[lane + 64 * p] : 0.0;
+  ask_queries(0);
+
+  const int u_to = idle ? 0 : min(first + min((split + 1) * chunk, units), hi_max / UNIT + 1);
+  const int u_from = max(first + split * chunk, low(hi_min) / UNIT) + (SHARE ? wave : 0);
+  constexpr int STEP = SHARE ? NW : 1;
+  const Constant<int> table = (Constant<int>)(uintptr_t)(a.table + (size_t)t.seq * a.table_ld);
+  const int lo_tile = low(hi_min), lo_most = low(hi_max), per_page = s.page / UNIT, scales_per_page = s.page / s.block;
+  // keys and values of a group are asked for as soon as those of the one before have been used, its page two groups ahead; pages and scales by scalar loads
+  uint4 kr[4][DP / 64], vr[VP / 16];
+  auto page_at = [&](int u) { return table[quotient(min(u, u_to - 1), a.per_page)]; };
+  auto in_page = [&](int u) { return (u - quotient(u, a.per_page) * per_page) * UNIT; };
+  auto head_of = [&](int id) { return (size_t)(page_ok(id, a.pages) ? id : 0) * s.kv_heads + head; };
+  auto load_k = [&](int u, int id) {
+    const uint8_t *const k = a.k + (head_of(id) * s.page + in_page(u)) * DP + lc * DP + lq * 16;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int j = 0; j < DP / 64; ++j) kr[tt][j] = *(const uint4 *)(k + tt * 16 * DP + j * 64);
+  };
+  auto load_v = [&](int u, int id) {
+    const uint8_t *const v = a.v + (head_of(id) * s.page + in_page(u)) * VP + lc * UNIT + lq * 16;
+#pragma unroll
+    for (int i = 0; i < VP / 16; ++i) vr[i] = *(const uint4 *)(v + i * 16 * UNIT);
+  };
+  // scales of the four blocks of 16 of a group
+  auto load_scales = [&](int u, int id) {
+    const size_t at = head_of(id) * scales_per_page;
+    const Constant<uint32_t> k = (Constant<uint32_t>)(uintptr_t)(a.ks + at), v = (Constant<uint32_t>)(uintptr_t)(a.vs + at);
+    Scales r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = (in_page(u) + i * 16) >> a.block_bits;
+      r.k[i] = k[j];
+      r.v[i] = v[j];
+    }
+    return r;
+  };
+  int id = 0, next = 0;
+  Scales sc = {};
+  if (u_from < u_to) {
+    id = page_at(u_from);
+    next = page_at(u_from + STEP);
+    load_k(u_from, id);
+    load_v(u_from, id);
+    sc = load_scales(u_from, id);
+  }
+
   h8 q[NQ][DP / 32], ql[F32 ? NQ : 1][F32 ? DP / 32 : 1];
   float qf[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     float *const rows = lds + (SHARE ? 0 : wave * 16 * FM::QLD);
-    for (int i = SHARE ? threadIdx.x : lane; i < 16 * (DP / 2); i += SHARE ? FM::THREADS : 64) {
-      const int c = min(c0 + n * 16 + i / (DP / 2), R - 1), p = i % (DP / 2), at = c / g;
-      const int2 d = pair_of(p, s.rot, s.pairs);
-      const float *const x = a.proj + (size_t)(t.r.first + at) * a.proj_ld + a.q_off + (size_t)(head * g + c - at * g) * s.dim;
-      float u = d.x < s.dim ? x[d.x] : 0.0f, v = d.y < s.dim ? x[d.y] : 0.0f;
-      if (p < s.rot / 2) {
-        float quarters, cs, sn;
-        int whole;
-        quarters_of(a.turn[p], pos + at, quarters, whole);
-        turned(quarters, whole, cs, sn);
-        const float y = u * cs - v * sn;
-        v = u * sn + v * cs;
-        u = y;
+    if (n) ask_queries(n);
+    int turned_at = -1;
+    float cs[PP], sn[PP];
+#pragma unroll
+    for (int k = 0; k < MINE; ++k) {
+      const int at = row_of(column(n, k));
+      if (at != turned_at) {
+        turned_at = at;
+#pragma unroll
+        for (int p = 0; p < PP; ++p) {
+          float quarters;
+          int whole;
+          quarters_of(turn[p], pos + at, quarters, whole);
+          turned(quarters, whole, cs[p], sn[p]);
+        }
       }
-      rows[i / (DP / 2) * FM::QLD + d.x] = u;
-      rows[i / (DP / 2) * FM::QLD + d.y] = v;
+#pragma unroll
+      for (int p = 0; p < PP; ++p) {
+        if (lane + 64 * p >= DP / 2) continue;
+        const int2 d = pair_of(lane + 64 * p, s.rot, s.pairs);
+        const float u = qx[k][p][0], v = qx[k][p][1];
+        const bool turns = lane + 64 * p < s.rot / 2;
+        float *const row = rows + (SHARE ? k * NW + wave : k) * FM::QLD;
+        row[d.x] = turns ? u * cs[p] - v * sn[p] : u;
+        row[d.y] = turns ? u * sn[p] + v * cs[p] : v;
+      }
     }
     __syncthreads();
     float most = 0.0f;
@@ -145,73 +240,26 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
     for (int v = 0; v < VP / 16; ++v) o[n][v] = f4{0, 0, 0, 0};
   }
 
-  const int u_to = min(first + min((split + 1) * chunk, units), hi_max / UNIT + 1);
-  const int u_from = max(first + split * chunk, low(hi_min) / UNIT) + (SHARE ? wave : 0);
-  constexpr int STEP = SHARE ? NW : 1;
-  const int *const table = a.table + (size_t)t.seq * a.table_ld;
-  const int lo_tile = low(hi_min), lo_most = low(hi_max);
-  uint4 kr[4][DP / 64];
-  auto page_at = [&](int u) { return __builtin_amdgcn_readfirstlane(table[min(u, u_to - 1) * UNIT / s.page]); };
-  auto head_of = [&](int id) { return (size_t)(page_ok(id, a.pages) ? id : 0) * s.kv_heads + head; };
-  auto load_k = [&](int u, int id) {
-    const uint8_t *const k = a.k + (head_of(id) * s.page + u * UNIT % s.page) * DP + lc * DP + lq * 16;
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int j = 0; j < DP / 64; ++j) kr[tt][j] = *(const uint4 *)(k + tt * 16 * DP + j * 64);
-  };
-  int id = 0, next = 0;
-  if (u_from < u_to && !idle) {
-    id = page_at(u_from);
-    next = page_at(u_from + STEP);
-    load_k(u_from, id);
-  }
-  for (int u = u_from; u < u_to && !idle; u += STEP) {
+  // a group, SUB blocks of 16 at a time
+  constexpr int SUB = FM::SUB;
+  for (int u = u_from; u < u_to; u += STEP) {
     const bool there = page_ok(id, a.pages);
-    const size_t at = head_of(id);
-    const int in = u * UNIT % s.page, base = u * UNIT;
-    uint4 vr[VP / 16];
-    {
-      const uint8_t *const v = a.v + (at * s.page + in) * VP + lc * UNIT + lq * 16;
-#pragma unroll
-      for (int i = 0; i < VP / 16; ++i) vr[i] = *(const uint4 *)(v + i * 16 * UNIT);
-    }
-    const bool whole = there && base + UNIT - 1 <= hi_min && base >= lo_most;
-    float kc[4], ve[4], vi[4];
+    const int base = u * UNIT, after = page_at(u + 2 * STEP);
+    const bool whole = there & (base + UNIT - 1 <= hi_min) & (base >= lo_most);  // every column sees all of it
+    uint32_t ks[4], vs[4];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
-      const size_t sc = at * (s.page / s.block) + (in + tt * 16) / s.block;
-      uint32_t ks = kx_f32_bits(a.ks[sc]), vs = kx_f32_bits(a.vs[sc]);
-      // blocks that no column sees may hold anything
-      if (!whole && (!there || base + tt * 16 > hi_max || base + tt * 16 + 15 < lo_tile)) ks = vs = kx_f32_bits(1.0f);
-      kc[tt] = kx_bits_f32(ks);
-      ve[tt] = (float)scale_exponent(vs);
-      vi[tt] = kx_bits_f32(scale_bits(-scale_exponent(vs)));
+      ks[tt] = sc.k[tt];
+      vs[tt] = sc.v[tt];
     }
-    f4 x[NQ][4];
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) x[n][tt] = f4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < DP / 64; ++j) {
-        const h8 k0 = unpacked(kr[tt][j].x, kr[tt][j].y), k1 = unpacked(kr[tt][j].z, kr[tt][j].w);
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          x[n][tt] = mfma(k0, q[n][2 * j], x[n][tt]);
-          x[n][tt] = mfma(k1, q[n][2 * j + 1], x[n][tt]);
-          if constexpr (F32) {
-            x[n][tt] = mfma(k0, ql[n][2 * j], x[n][tt]);
-            x[n][tt] = mfma(k1, ql[n][2 * j + 1], x[n][tt]);
-          }
-        }
-      }
-    }
-    id = next;
-    if (u + STEP < u_to) load_k(u + STEP, id);
-    next = page_at(u + 2 * STEP);
     bool nan = false;
     if (!whole) {
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {  // blocks that no column sees may hold anything
+        const bool unseen = !there | (base + tt * 16 > hi_max) | (base + tt * 16 + 15 < lo_tile);
+        ks[tt] = unseen ? 0x3f800000u : ks[tt];
+        vs[tt] = unseen ? 0x3f800000u : vs[tt];
+      }
       if (!there && lane == 0) atomicOr(a.fault, BAD_PAGE);
 #pragma unroll
       for (int d = 0; d < 4; ++d) {  // values that no column sees, and NaN, become zero
@@ -228,76 +276,119 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
         }
       }
     }
-    h8 ph[NQ][2], pl[F32 ? NQ : 1][2];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float most = NONE;
+    for (int t0 = 0; t0 < 4; t0 += SUB) {
+      f4 x[NQ][SUB];
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const float f = qf[n] * kc[tt];
+      for (int tt = 0; tt < SUB; ++tt) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float y = __builtin_fmaf(x[n][tt][i], f, ve[tt]);
-          if (!whole) {
-            const int j = base + tt * 16 + lq * 4 + i;
-            if (!there || j > hi[n] || j < lo[n]) y = -__builtin_inff();
+        for (int n = 0; n < NQ; ++n) x[n][tt] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < DP / 64; ++j) {
+          const h8 k0 = unpacked(kr[t0 + tt][j].x, kr[t0 + tt][j].y), k1 = unpacked(kr[t0 + tt][j].z, kr[t0 + tt][j].w);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            x[n][tt] = mfma(k0, q[n][2 * j], x[n][tt]);
+            x[n][tt] = mfma(k1, q[n][2 * j + 1], x[n][tt]);
+            if constexpr (F32) {
+              x[n][tt] = mfma(k0, ql[n][2 * j], x[n][tt]);
+              x[n][tt] = mfma(k1, ql[n][2 * j + 1], x[n][tt]);
+            }
           }
-          x[n][tt][i] = y;
-          most = fmaxf(most, y);
         }
       }
-      most = fmaxf(m[n], quarters_max(most));
-      if (__builtin_amdgcn_ballot_w64(most > m[n])) {
-        const float f = exp2_(m[n] - most);
-        m[n] = most;
-        l[n] *= f;
-#pragma unroll
-        for (int v = 0; v < VP / 16; ++v) o[n][v] *= f;
+      if (t0 + SUB == 4 && u + STEP < u_to) {
+        load_k(u + STEP, next);
+        sc = load_scales(u + STEP, next);
       }
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = exp2_(x[n][tt][i] - m[n]);
-          sum += p;
-          const _Float16 h = (_Float16)p;
-          ph[n][tt >> 1][(tt & 1) * 4 + i] = h;
-          if constexpr (F32) pl[n][tt >> 1][(tt & 1) * 4 + i] = (_Float16)(p - (float)h);
-        }
-        l[n] = __builtin_fmaf(sum, vi[tt], l[n]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < VP / 16; ++i) {
-      const h8 v0 = unpacked(vr[i].x, vr[i].y), v1 = unpacked(vr[i].z, vr[i].w);
+      h8 ph[NQ][SUB / 2], pl[F32 ? NQ : 1][SUB / 2];
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
-        o[n][i] = mfma(v0, ph[n][0], o[n][i]);
-        o[n][i] = mfma(v1, ph[n][1], o[n][i]);
-        if constexpr (F32) {
-          o[n][i] = mfma(v0, pl[n][0], o[n][i]);
-          o[n][i] = mfma(v1, pl[n][1], o[n][i]);
+#pragma unroll
+        for (int tt = 0; tt < SUB; ++tt) {
+          const float f = qf[n] * kx_bits_f32(ks[t0 + tt]), e = (float)scale_exponent(vs[t0 + tt]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[n][tt][i] = __builtin_fmaf(x[n][tt][i], f, e);
+        }
+        if (!whole) {
+          // positions of the lane's tokens that its column sees, counted from its first token
+          const int from = there ? lo[n] - (base + t0 * 16 + lq * 4) : 1 << 30, to = hi[n] - (base + t0 * 16 + lq * 4);
+#pragma unroll
+          for (int tt = 0; tt < SUB; ++tt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[n][tt][i] = ((tt * 16 + i > to) | (tt * 16 + i < from)) ? -__builtin_inff() : x[n][tt][i];
+        }
+        float most = NONE;
+#pragma unroll
+        for (int tt = 0; tt < SUB; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) most = fmaxf(most, x[n][tt][i]);
+        most = fmaxf(m[n], quarters_max(most));
+        if (__builtin_amdgcn_ballot_w64(most > m[n])) {
+          const float f = exp2_(m[n] - most);
+          m[n] = most;
+          l[n] *= f;
+#pragma unroll
+          for (int v = 0; v < VP / 16; ++v) o[n][v] *= f;
+        }
+#pragma unroll
+        for (int tt = 0; tt < SUB; ++tt) {
+          f4 p;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] = exp2_(x[n][tt][i] - m[n]);
+          l[n] = __builtin_fmaf((p[0] + p[1]) + (p[2] + p[3]), kx_bits_f32(scale_bits(-scale_exponent(vs[t0 + tt]))), l[n]);
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const h2 h = halves_of(p[i], p[i + 1]);
+            ph[n][tt >> 1][(tt & 1) * 4 + i] = h[0];
+            ph[n][tt >> 1][(tt & 1) * 4 + i + 1] = h[1];
+            if constexpr (F32) {
+              const h2 r = halves_of(p[i] - (float)h[0], p[i + 1] - (float)h[1]);
+              pl[n][tt >> 1][(tt & 1) * 4 + i] = r[0];
+              pl[n][tt >> 1][(tt & 1) * 4 + i + 1] = r[1];
+            }
+          }
         }
       }
-    }
-    if (__builtin_amdgcn_ballot_w64(nan)) {  // NaN among the values: the columns that see it have it
-      const uint8_t *const v = a.v + (at * s.page + in) * VP;
 #pragma unroll
       for (int i = 0; i < VP / 16; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint8_t *const row = v + (i * 16 + lq * 4 + e) * UNIT;
-#pragma unroll 1
-          for (int p = 0; p < UNIT; ++p)
-            if ((row[p] & 0x7f) == 0x7f) {
-              const int j = base + token_of(p);
+        for (int h = 0; h < SUB / 2; ++h) {
+          const h8 v = t0 / 2 + h == 0 ? unpacked(vr[i].x, vr[i].y) : unpacked(vr[i].z, vr[i].w);
 #pragma unroll
-              for (int n = 0; n < NQ; ++n)
-                if (j <= hi[n] && j >= lo[n]) o[n][i][e] = __builtin_nanf("");
-            }
+          for (int n = 0; n < NQ; ++n) {
+            o[n][i] = mfma(v, ph[n][h], o[n][i]);
+            if constexpr (F32) o[n][i] = mfma(v, pl[n][h], o[n][i]);
+          }
         }
     }
+    if (u + STEP < u_to) load_v(u + STEP, next);
+    if (!whole)
+      if (__builtin_amdgcn_ballot_w64(nan)) {  // NaN among the values: the columns that see it, which products of ones and zeros say, have it
+        const uint8_t *const v = a.v + (head_of(id) * s.page + in_page(u)) * VP + lc * UNIT + lq * 16;
+        h8 sees[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int j = base + (e >> 2) * 16 + lq * 4 + (e & 3);
+            sees[n][e >> 3][e & 7] = ((j <= hi[n]) & (j >= lo[n])) ? (_Float16)1.0f : (_Float16)0.0f;
+          }
+#pragma unroll
+        for (int i = 0; i < VP / 16; ++i) {
+          uint4 w = *(const uint4 *)(v + i * 16 * UNIT);
+          auto ones = [](uint32_t w) { return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0x38u; };
+          const h8 v0 = unpacked(ones(w.x), ones(w.y)), v1 = unpacked(ones(w.z), ones(w.w));
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            const f4 seen = mfma(v1, sees[n][1], mfma(v0, sees[n][0], f4{0, 0, 0, 0}));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][i][e] = seen[e] > 0.0f ? __builtin_nanf("") : o[n][i][e];
+          }
+        }
+      }
+    id = next;
+    next = after;
   }
 #pragma unroll
   for (int n = 0; n < NQ; ++n) l[n] = quarters_sum(l[n]);
@@ -305,7 +396,7 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
   // results: four neighbouring dimensions of a column at a time
   float *const part = a.part + (size_t)(task * s.kv_heads + head) * a.splits * FM::PART;
   auto give = [&](int c, int d, f4 y) {  // column c of the sequence, dimensions d .. d + 3
-    const int at = c / g;
+    const int at = row_of(c);
     const size_t to = (size_t)(t.r.first + at) * a.out_ld + (size_t)(head * g + c - at * g) * s.vdim + d;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -390,6 +481,7 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
   __syncthreads();
   if (!last) return;
   if (threadIdx.x == 0) kx_arrive_reset(arrived);
+  // weights of the parts, a wave a column and a lane a part; then their sums
   const int cols = min(COLS, R - w0);
   float2 *const st = (float2 *)lds;  // [used][COLS]
   for (int i = threadIdx.x; i < used * COLS; i += FM::THREADS)
@@ -398,26 +490,40 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
       st[i] = make_float2(kx_bits_f32((uint32_t)w), kx_bits_f32((uint32_t)(w >> 32)));
     }
   __syncthreads();
-  for (int c = threadIdx.x; c < cols; c += FM::THREADS) {
+  for (int c = wave; c < cols; c += NW) {
     float most = NONE, sum = 0.0f;
-    for (int p = 0; p < used; ++p) most = fmaxf(most, st[p * COLS + c].x);
-    for (int p = 0; p < used; ++p) sum = __builtin_fmaf(st[p * COLS + c].y, exp2_(st[p * COLS + c].x - most), sum);
+    for (int p = lane; p < used; p += 64) most = fmaxf(most, st[p * COLS + c].x);
+    most = kxw::wave_max_f32(most);
+    for (int p = lane; p < used; p += 64) sum = __builtin_fmaf(st[p * COLS + c].y, exp2_(st[p * COLS + c].x - most), sum);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-    for (int p = 0; p < used; ++p) st[p * COLS + c].x = exp2_(st[p * COLS + c].x - most) * f;
+    for (int p = lane; p < used; p += 64) st[p * COLS + c].x = exp2_(st[p * COLS + c].x - most) * f;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < cols * (VP / 4); i += FM::THREADS) {
     const int c = i / (VP / 4), d = i % (VP / 4) * 4;
     const uint64_t *from = (const uint64_t *)(part + (size_t)c * VP + d);
     f4 y = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int p = 0; p < used; ++p) {
-      const uint64_t x0 = kx_arrive_load(from + p * (FM::PART / 2)), x1 = kx_arrive_load(from + p * (FM::PART / 2) + 1);
-      const float f = st[p * COLS + c].x;
-      y[0] = __builtin_fmaf(kx_bits_f32((uint32_t)x0), f, y[0]);
-      y[1] = __builtin_fmaf(kx_bits_f32((uint32_t)(x0 >> 32)), f, y[1]);
-      y[2] = __builtin_fmaf(kx_bits_f32((uint32_t)x1), f, y[2]);
-      y[3] = __builtin_fmaf(kx_bits_f32((uint32_t)(x1 >> 32)), f, y[3]);
+    constexpr int AT_ONCE = 16;
+    for (int p0 = 0; p0 < used; p0 += AT_ONCE) {
+      uint64_t w[AT_ONCE][2];
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k)
+        if (p0 + k < used) {
+          const size_t at = (size_t)(p0 + k) * (FM::PART / 2);
+          w[k][0] = kx_arrive_load(from + at);
+          w[k][1] = kx_arrive_load(from + at + 1);
+        }
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        if (p0 + k >= used) continue;
+        const float f = st[(p0 + k) * COLS + c].x;
+        y[0] = __builtin_fmaf(kx_bits_f32((uint32_t)w[k][0]), f, y[0]);
+        y[1] = __builtin_fmaf(kx_bits_f32((uint32_t)(w[k][0] >> 32)), f, y[1]);
+        y[2] = __builtin_fmaf(kx_bits_f32((uint32_t)w[k][1]), f, y[2]);
+        y[3] = __builtin_fmaf(kx_bits_f32((uint32_t)(w[k][1] >> 32)), f, y[3]);
+      }
     }
     give(w0 + c, d, y);
   }
@@ -434,8 +540,11 @@ int launch(KxPagedArgs a, int g, hipStream_t st) {
   const long busy = (long)std::min(a.batch, a.tokens) * ((rows * g + FM::COLS - 1) / FM::COLS) * kv;  // workgroups of whole sequences
   const long room = std::min<long>({(long)(a.part_floats / FM::PART) / std::max<long>(1, tasks * kv), STATS / FM::COLS, units});
   const long want = ((long)cus * FM::WAVES + busy - 1) / busy;
-  a.splits = (int)std::max<long>(1, std::min(room, want));
+  // a part has a group for each wave at least, and where more than 256 columns of parts are for one workgroup to add up, eight
+  const long waves = FM::SHARE ? FM::NW : 1, most_parts = std::max(std::min<long>(units / waves, 256 / FM::COLS), units / (waves * 8));
+  a.splits = (int)std::max<long>(1, std::min({room, want, most_parts}));
   a.chunk = (units + a.splits - 1) / a.splits;
+  a.by_splits = divider(a.splits);
   // a sequence longer than `longest` has longer parts
   attend_k<FM><<<dim3((unsigned)(tasks * a.splits * kv)), FM::THREADS, 0, st>>>(a);
   KX_LAUNCH_CHECK();
@@ -446,9 +555,10 @@ template <int DP, int VP, bool F32>
 int launch_columns(const KxPagedArgs &a, hipStream_t st) {
   const int g = a.s.heads / a.s.kv_heads;
   const long columns = (long)a.tokens * g / std::min(a.batch, a.tokens);  // of a sequence, on average
+  constexpr int NQ = DP == 256 ? 1 : 2;  // the widest rows leave registers for one block of columns
   if (columns <= 16) return launch<Form<DP, VP, 1, true, F32>>(a, g, st);
-  if (columns <= 64) return launch<Form<DP, VP, 2, true, F32>>(a, g, st);
-  return launch<Form<DP, VP, 2, false, F32>>(a, g, st);
+  if (columns <= 64) return launch<Form<DP, VP, NQ, true, F32>>(a, g, st);
+  return launch<Form<DP, VP, NQ, false, F32>>(a, g, st);
 }
 template <bool F32>
 int launch_widths(const KxPagedArgs &a, hipStream_t st) {

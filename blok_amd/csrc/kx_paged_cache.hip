@@ -349,6 +349,8 @@ extern "C" int kx_paged_create(const kx_paged_config *c, const double *h_freq, i
     s.size = c->size; s.scale = c->scale;
     const kxpage::Widths w = kxpage::widths_of(c->dim, c->vdim);
     s.dp = w.k; s.vp = w.v;
+    p->a.by_g = divider(s.heads / s.kv_heads); p->a.by_kv = divider(s.kv_heads); p->a.per_page = divider(s.page / UNIT);
+    p->a.block_bits = __builtin_ctz((unsigned)s.block);
     p->f32 = f32 != 0;
     p->max_batch = max_batch; p->max_tokens = max_tokens;
     p->a.arrivals = kx_paged_arrivals(s, max_batch, max_tokens);
