@@ -1,12 +1,12 @@
 // kx_paged_cache.hip -- keys and values into the pages of an 8-bit cache and out of them again (kx_paged.h).  No counterpart in the reference,
 // which stores 32-bit keys and values tile by tile on a disk (KvCache, src/kimi_exec.cu:192-238).
 //
-// append: a workgroup has the new tokens that lie in one group of 64 of a sequence, for one head of keys and values.  Every element is read once, turned by
-//   its position in 64 bits and kept as a float whose last bit says whether anything was cut off; rounding that to 4 bits of fraction at any scale is
-//   one rounding of the exact number.  The largest magnitude of each block goes through LDS; with the scales known, codes are made in registers.
-//   A few tokens whose blocks keep their scales are stored byte by byte (a byte of a row of 64 for each value: 128 of them for a decoded token).
-//   Otherwise the group is put together in LDS, with the tokens that it keeps, and written in whole pieces of 16 bytes.
-// read: the same groups, codes times scales as bf16, which holds them exactly.
+// append: a workgroup has the new tokens that lie in one group of 64 of a sequence, for one head of keys and values, and wave w of its four the tokens whose
+//   values are bytes 16 w .. 16 w + 15 of a row: 16 j + 4 w + r.  Every element is read once, turned by its position in 64 bits -- three sines and cosines a
+//   lane, the others by addition of angles -- and kept as a float whose last bit says whether anything was cut off; rounding that to 4 bits of fraction at any
+//   scale is one rounding of the exact number.  The largest magnitude of each block goes through LDS; with the scales known, codes are made in registers and
+//   go straight to the pages: keys a row at a time, values 16 bytes of a row at a time, with the older ones of those 16 where there are any.
+// read: the same groups, codes times scales as bf16, which holds them exactly; values are turned four tokens by eight dimensions a lane.
 #include <algorithm>
 #include <cmath>
 #include <memory>
@@ -15,22 +15,22 @@
 #include "kx_common.h"
 #include "kx_math.h"
 #include "kx_paged.h"
+#include "kx_wave.h"
 
 namespace {
 
 using namespace kxpage;
 
-constexpr int THREADS = 256, FEW = 4;  // FEW: most tokens that are stored byte by byte
+constexpr int THREADS = 256, FEW = 4;  // FEW: most tokens whose values are stored byte by byte
 
-// x with its last bits cut off, and the last that is left set where that changed anything
+// x with its last bits cut off, and the last that is left set where that changed anything; less than any code can hold becomes zero
 __device__ __forceinline__ float sticky(double x) {
-  float f = (float)x;
-  if ((double)f != x && f == f) {
-    uint32_t u = kx_f32_bits(f);
-    if (__builtin_fabs((double)f) > __builtin_fabs(x)) --u;
-    f = kx_bits_f32(u | 1u);
-  }
-  return f;
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  const uint32_t hi = (uint32_t)(u >> 32), size = hi & 0x7fffffffu;
+  uint32_t f = (uint32_t)(u >> 29) - (896u << 23) | ((uint32_t)u & 0x1fffffffu ? 1u : 0u);
+  f = size < 897u << 20 ? 0u : size >= 1151u << 20 ? 0x7f7fffffu : f & 0x7fffffffu;
+  f = size >= 0x7ff00000u ? 0x7fc00000u : f;
+  return kx_bits_f32(f | (hi & 0x80000000u));
 }
 __device__ __forceinline__ uint32_t magnitude(float x) {  // bits of |x|; 0 for what is not finite
   const uint32_t u = kx_f32_bits(x) & 0x7fffffffu;
@@ -40,11 +40,6 @@ __device__ __forceinline__ uint32_t magnitude(float x) {  // bits of |x|; 0 for 
 __device__ __forceinline__ uint32_t codes(float a, float b, float inverse) {
   auto scaled = [&](float x) { return (kx_f32_bits(x) & 0x7f800000u) == 0x7f800000u ? __builtin_nanf("") : x * inverse; };
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(scaled(a), scaled(b), 0, false) & 0xffffu;
-}
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
-  return v;
 }
 // the four codes of a word divided by 2^down
 __device__ __forceinline__ uint32_t lowered(uint32_t w, int down) {
@@ -57,215 +52,273 @@ __device__ __forceinline__ uint32_t lowered(uint32_t w, int down) {
 }
 
 struct Unit {
-  int seq, from, to, row;  // new tokens of the group [from, to), rows of the first
-  size_t head;             // (page * kv_heads + head)
-  int in_page;             // position of the group in its page
-  int pos;                 // of the group
-  bool ok;
+  int from, to, row;  // new tokens of the group [from, to), row of the first; none: to is 0
+  size_t head;        // page * kv_heads + head
+  int in_page;        // position of the group in its page
+  int pos, id;        // of the group; its page, which need not exist
 };
 __device__ __forceinline__ Unit unit_of(const KxPagedArgs &a) {
   const Task t = find_task(a, blockIdx.x, [](const Rows &r) { return units_of(r.pos, r.n); });
   Unit u;
-  u.ok = t.r.n > 0;
-  if (!u.ok) return u;
-  u.seq = t.seq;
   u.pos = (t.r.pos / UNIT + t.index) * UNIT;
   u.from = max(t.r.pos - u.pos, 0);
-  u.to = min(t.r.pos + t.r.n - u.pos, UNIT);
+  u.to = t.r.n > 0 ? min(t.r.pos + t.r.n - u.pos, UNIT) : 0;
+  if (!u.to) return u;
   u.row = t.r.first + u.pos + u.from - t.r.pos;
-  const int id = a.table[(size_t)t.seq * a.table_ld + u.pos / a.s.page];
-  if (!page_ok(id, a.pages)) {
-    if (threadIdx.x == 0) atomicOr(a.fault, BAD_PAGE);
-    u.ok = false;
-    return u;
-  }
-  u.head = (size_t)id * a.s.kv_heads + blockIdx.y;
-  u.in_page = u.pos % a.s.page;
+  const int page = quotient(u.pos / UNIT, a.per_page);
+  u.id = a.table[(size_t)t.seq * a.table_ld + page];
+  u.in_page = u.pos - page * a.s.page;
   return u;
+}
+__device__ __forceinline__ bool placed(const KxPagedArgs &a, Unit &u) {  // whether the page exists
+  u.head = (size_t)u.id * a.s.kv_heads + blockIdx.y;
+  if (page_ok(u.id, a.pages)) return true;
+  if (threadIdx.x == 0) atomicOr(a.fault, BAD_PAGE);
+  return false;
+}
+// bytes of a word of tokens t .. t + 3 that lie in [from, to)
+__device__ __forceinline__ uint32_t bytes_within(int t, int from, int to) {
+  const int n = max(min(to - t, 4), 0), k = max(min(from - t, 4), 0);
+  return (n == 4 ? ~0u : (1u << 8 * n) - 1u) & (k == 4 ? 0u : ~0u << 8 * k);
 }
 
 template <int DP, int VP>
 __global__ void __launch_bounds__(THREADS) append_k(KxPagedArgs a) {
-  constexpr int PK = (DP + 127) / 128, PV = (VP + 127) / 128;  // pairs of a lane
-  __shared__ __attribute__((aligned(16))) uint8_t lk[UNIT * DP], lv[VP * UNIT];
+  constexpr int PK = (DP + 127) / 128, PV = VP / 64;  // of a lane: pairs of a key, elements of a value
   __shared__ uint32_t most[4][8];
   const KxPagedSpec &s = a.s;
-  const Unit u = unit_of(a);
-  if (!u.ok) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, from = u.from, to = u.to;
-  uint8_t *const gk = a.k + (u.head * s.page + u.in_page) * DP, *const gv = a.v + (u.head * s.page + u.in_page) * VP;
-  const size_t sc = u.head * (s.page / s.block) + u.in_page / s.block;  // scale of the group's first block
-  const int b0 = from / s.block;
-  const bool kept = from % s.block != 0;  // the first block has older tokens
-  const int old_k = kept ? scale_exponent(kx_f32_bits(a.ks[sc + b0])) : 0, old_v = kept ? scale_exponent(kx_f32_bits(a.vs[sc + b0])) : 0;
-
-  // wave w has tokens w, w + 4, ... of the group; four of them are in a block of 16
-  float xk[16][PK][2], xv[16][PV][2];
+  Unit u = unit_of(a);
+  if (!u.to) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), from = u.from, to = u.to, t0 = 4 * wave;
+  auto fresh = [&](int j, int r) { return t0 + 16 * j + r >= from && t0 + 16 * j + r < to; };
+  float xk[4][4][PK][2], xv[4][4][PV];
   double turn[PK];
 #pragma unroll
   for (int p = 0; p < PK; ++p) turn[p] = lane + 64 * p < s.rot / 2 ? a.turn[lane + 64 * p] : 0.0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+      for (int p = 0; p < PK; ++p) xk[j][r][p][0] = xk[j][r][p][1] = 0.0f;
+#pragma unroll
+      for (int p = 0; p < PV; ++p) xv[j][r][p] = 0.0f;
+      if (!fresh(j, r)) continue;
+      const float *const row = a.proj + (size_t)(u.row + t0 + 16 * j + r - from) * a.proj_ld;
+      const float *const rk = row + a.k_off + (size_t)blockIdx.y * s.dim, *const rv = row + a.v_off + (size_t)blockIdx.y * s.vdim;
+#pragma unroll
+      for (int p = 0; p < PK; ++p) {
+        const int2 d = pair_of(lane + 64 * p, s.rot, s.pairs);
+        if (d.x < s.dim) xk[j][r][p][0] = rk[d.x];
+        if (d.y < s.dim) xk[j][r][p][1] = rk[d.y];
+      }
+#pragma unroll
+      for (int p = 0; p < PV; ++p)
+        if (lane + 64 * p < s.vdim) xv[j][r][p] = rv[lane + 64 * p];
+    }
+  if (!placed(a, u)) return;
+  uint8_t *const gk = a.k + (u.head * s.page + u.in_page) * DP, *const gv = a.v + (u.head * s.page + u.in_page) * VP;
+  const size_t sc = u.head * (s.page >> a.block_bits) + (u.in_page >> a.block_bits);  // scale of the group's first block
+  const int b0 = from >> a.block_bits, per = s.block / 16;
+  const bool kept = (from & (s.block - 1)) != 0;  // the first block has older tokens
+  const int old_k = kept ? scale_exponent(kx_f32_bits(a.ks[sc + b0])) : 0, old_v = kept ? scale_exponent(kx_f32_bits(a.vs[sc + b0])) : 0;
+
+  // turns: of the wave's first four tokens with new ones among them, of one token, of 16
+  const bool single = to - from == 1;
+  const int j0 = (from - t0 + 12) >> 4;
+  double c0[PK], s0[PK], c1[PK], s1[PK], c16[PK], s16[PK];
+#pragma unroll
+  for (int p = 0; p < PK; ++p) {
+    auto eval = [&](int n, double &c, double &s) {
+      const double at = turn[p] * (double)n;
+      turned(at - __builtin_rint(at), c, s);
+    };
+    c1[p] = c16[p] = 1.0;
+    s1[p] = s16[p] = 0.0;
+    eval(u.pos + (single ? from : t0 + 16 * j0), c0[p], s0[p]);
+    if (!single) eval(1, c1[p], s1[p]);
+    if (to - from > 4) eval(16, c16[p], s16[p]);
+  }
   uint32_t mk[4] = {0, 0, 0, 0}, mv[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int t = wave + 4 * i;
-    const bool mine = t >= from && t < to;
-    const float *row = a.proj + (size_t)(u.row + (mine ? t - from : 0)) * a.proj_ld;
-    const float *rk = row + a.k_off + (size_t)blockIdx.y * s.dim, *rv = row + a.v_off + (size_t)blockIdx.y * s.vdim;
+  for (int j = 0; j < 4; ++j) {
+    if (j < j0 || t0 + 16 * j >= to) continue;
 #pragma unroll
     for (int p = 0; p < PK; ++p) {
-      const int2 d = pair_of(lane + 64 * p, s.rot, s.pairs);
-      xk[i][p][0] = mine && d.x < s.dim ? rk[d.x] : 0.0f;
-      xk[i][p][1] = mine && d.y < s.dim ? rk[d.y] : 0.0f;
-    }
+      double c = c0[p], n = s0[p];
 #pragma unroll
-    for (int p = 0; p < PV; ++p) {
-      const int d = 2 * (lane + 64 * p);
-      xv[i][p][0] = mine && d < s.vdim ? rv[d] : 0.0f;
-      xv[i][p][1] = mine && d + 1 < s.vdim ? rv[d + 1] : 0.0f;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int t = wave + 4 * i;
-    if (t < from || t >= to) continue;
-#pragma unroll
-    for (int p = 0; p < PK; ++p) {
-      if (lane + 64 * p < s.rot / 2) {
-        double c, n;
-        const double at = turn[p] * (double)(u.pos + t);
-        turned(at - __builtin_rint(at), c, n);
-        const double x = xk[i][p][0], y = xk[i][p][1];
-        xk[i][p][0] = sticky(x * c - y * n);
-        xk[i][p][1] = sticky(x * n + y * c);
+      for (int r = 0; r < 4; ++r) {
+        if (fresh(j, r)) {
+          float &x = xk[j][r][p][0], &y = xk[j][r][p][1];
+          if (lane + 64 * p < s.rot / 2) {
+            const double x0 = x, y0 = y;
+            x = sticky(x0 * c - y0 * n);
+            y = sticky(x0 * n + y0 * c);
+          }
+          mk[j] = max(mk[j], max(magnitude(x), magnitude(y)));
+        }
+        if (r < 3 && !single) {
+          const double d = c * c1[p] - n * s1[p];
+          n = c * s1[p] + n * c1[p];
+          c = d;
+        }
       }
-      mk[i >> 2] = max(mk[i >> 2], max(magnitude(xk[i][p][0]), magnitude(xk[i][p][1])));
+      const double d = c0[p] * c16[p] - s0[p] * s16[p];
+      s0[p] = c0[p] * s16[p] + s0[p] * c16[p];
+      c0[p] = d;
     }
 #pragma unroll
-    for (int p = 0; p < PV; ++p) mv[i >> 2] = max(mv[i >> 2], max(magnitude(xv[i][p][0]), magnitude(xv[i][p][1])));
-  }
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    mk[g] = wave_max(mk[g]);
-    mv[g] = wave_max(mv[g]);
+      for (int p = 0; p < PV; ++p) mv[j] = max(mv[j], magnitude(xv[j][r][p]));
+    mk[j] = kx_f32_bits(kxw::wave_max_f32(kx_bits_f32(mk[j])));
+    mv[j] = kx_f32_bits(kxw::wave_max_f32(kx_bits_f32(mv[j])));
   }
   if (lane == 0) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      most[wave][g] = mk[g];
-      most[wave][4 + g] = mv[g];
+    for (int j = 0; j < 4; ++j) {
+      most[wave][j] = mk[j];
+      most[wave][4 + j] = mv[j];
     }
   }
   __syncthreads();
   // exponents of the blocks that the group's four blocks of 16 lie in
   int ek[4], ev[4];
-  const int per = s.block / 16;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    uint32_t k = 0, v = 0;
+  for (int j = 0; j < 4; ++j) {
+    mk[j] = max(max(most[0][j], most[1][j]), max(most[2][j], most[3][j]));
+    mv[j] = max(max(most[0][4 + j], most[1][4 + j]), max(most[2][4 + j], most[3][4 + j]));
+  }
 #pragma unroll
-    for (int h = 0; h < 4; ++h)
-      if (h / per == g / per) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          k = max(k, most[w][h]);
-          v = max(v, most[w][4 + h]);
-        }
-      }
-    ek[g] = exponent_of(k);
-    ev[g] = exponent_of(v);
-    if (kept && g / per == b0) {
-      ek[g] = max(ek[g], old_k);
-      ev[g] = max(ev[g], old_v);
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t k2 = max(mk[j & 2], mk[j | 1]), v2 = max(mv[j & 2], mv[j | 1]), k4 = max(max(mk[0], mk[1]), max(mk[2], mk[3])), v4 = max(max(mv[0], mv[1]), max(mv[2], mv[3]));
+    ek[j] = exponent_of(per == 1 ? mk[j] : per == 2 ? k2 : k4);
+    ev[j] = exponent_of(per == 1 ? mv[j] : per == 2 ? v2 : v4);
+    if (kept && j / per == b0) {
+      ek[j] = max(ek[j], old_k);
+      ev[j] = max(ev[j], old_v);
     }
   }
   // the exponents of the first block that the group writes to
   const int g0 = b0 * per, ek0 = g0 == 0 ? ek[0] : g0 == 1 ? ek[1] : g0 == 2 ? ek[2] : ek[3], ev0 = g0 == 0 ? ev[0] : g0 == 1 ? ev[1] : g0 == 2 ? ev[2] : ev[3];
   const int grown_k = kept ? ek0 - old_k : 0, grown_v = kept ? ev0 - old_v : 0;
-  if (tid < 4 && tid % per == 0 && tid / per >= b0 && tid / per <= (to - 1) / s.block) {
+  if (tid < 4 && (tid & (per - 1)) == 0 && tid / per >= b0 && tid / per <= (to - 1) >> a.block_bits) {
     const int k = tid == 0 ? ek[0] : tid == 1 ? ek[1] : tid == 2 ? ek[2] : ek[3], v = tid == 0 ? ev[0] : tid == 1 ? ev[1] : tid == 2 ? ev[2] : ev[3];
     a.ks[sc + tid / per] = kx_bits_f32(scale_bits(k));
     a.vs[sc + tid / per] = kx_bits_f32(scale_bits(v));
   }
-  const bool few = to - from <= FEW && !grown_k && !grown_v;
-  if (!few) {
-    if (from > 0) {  // what the group keeps
-      for (int i = tid; i < from * DP / 16; i += THREADS) ((uint4 *)lk)[i] = ((const uint4 *)gk)[i];
-      for (int i = tid; i < VP * UNIT / 16; i += THREADS) ((uint4 *)lv)[i] = ((const uint4 *)gv)[i];
-      __syncthreads();
-      if (grown_k)
-        for (int i = tid + b0 * s.block * DP / 4; i < from * DP / 4; i += THREADS) ((uint32_t *)lk)[i] = lowered(((uint32_t *)lk)[i], grown_k);
-      if (grown_v)
-        for (int i = tid; i < VP * UNIT / 4; i += THREADS) {  // a word has four tokens of one block of 16
-          const int t = token_of(i * 4 % UNIT);
-          if (t / s.block == b0) ((uint32_t *)lv)[i] = lowered(((uint32_t *)lv)[i], grown_v);
+
+  // keys
+  if (grown_k) {
+    uint32_t *const w = (uint32_t *)(gk + b0 * s.block * DP);
+    for (int i = tid; i < (from - b0 * s.block) * (DP / 4); i += THREADS) w[i] = lowered(w[i], grown_k);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float rk = kx_bits_f32(scale_bits(-ek[j]));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (!fresh(j, r)) continue;
+      uint8_t *const row = gk + (t0 + 16 * j + r) * DP;
+#pragma unroll
+      for (int p = 0; p < PK; ++p)
+        if (lane + 64 * p < DP / 2) {
+          const int2 d = pair_of(lane + 64 * p, s.rot, s.pairs);
+          const uint32_t c = codes(xk[j][r][p][0], xk[j][r][p][1], rk);
+          if (d.y == d.x + 1) {
+            *(uint16_t *)(row + d.x) = (uint16_t)c;
+          } else {
+            row[d.x] = (uint8_t)c;
+            row[d.y] = (uint8_t)(c >> 8);
+          }
         }
-    } else {
-      for (int i = tid; i < VP * UNIT / 16; i += THREADS) ((uint4 *)lv)[i] = make_uint4(0, 0, 0, 0);
     }
-    __syncthreads();
   }
-  uint8_t *const tk = few ? gk : lk, *const tv = few ? gv : lv;
+  // values
+  const bool any = j0 < 4 && t0 + 16 * j0 < to;
+  if (!any && !grown_v) return;
+  const bool few = to - from <= FEW && !grown_v, alone = from == 0 || (from <= t0 && to >= t0 + 52);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int t = wave + 4 * i;
-    if (t < from || t >= to) continue;
-    const float rk = kx_bits_f32(scale_bits(-ek[i >> 2])), rv = kx_bits_f32(scale_bits(-ev[i >> 2]));
-    const int at = place_of(t);
+  for (int p = 0; p < PV; ++p) {
+    uint8_t *const at = gv + (lane + 64 * p) * UNIT + 16 * wave;
+    uint32_t w[4];
 #pragma unroll
-    for (int p = 0; p < PK; ++p)
-      if (lane + 64 * p < DP / 2) {
-        const int2 d = pair_of(lane + 64 * p, s.rot, s.pairs);
-        const uint32_t c = codes(xk[i][p][0], xk[i][p][1], rk);
-        if (d.y == d.x + 1) {
-          *(uint16_t *)(tk + t * DP + d.x) = (uint16_t)c;
-        } else {
-          tk[t * DP + d.x] = (uint8_t)c;
-          tk[t * DP + d.y] = (uint8_t)(c >> 8);
-        }
+    for (int j = 0; j < 4; ++j) {
+      const float rv = kx_bits_f32(scale_bits(-ev[j]));
+      w[j] = codes(xv[j][0][p], xv[j][1][p], rv) | codes(xv[j][2][p], xv[j][3][p], rv) << 16;
+    }
+    if (few) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (fresh(j, r)) at[4 * j + r] = (uint8_t)(w[j] >> 8 * r);
+      continue;
+    }
+    if (!alone) {
+      const uint4 o = *(const uint4 *)at;
+      const uint32_t old[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t mask = bytes_within(t0 + 16 * j, from, to);
+        w[j] = (w[j] & mask) | ((grown_v && j / per == b0 ? lowered(old[j], grown_v) : old[j]) & ~mask);
       }
-#pragma unroll
-    for (int p = 0; p < PV; ++p)
-      if (lane + 64 * p < VP / 2) {
-        const int d = 2 * (lane + 64 * p);
-        const uint32_t c = codes(xv[i][p][0], xv[i][p][1], rv);
-        tv[d * UNIT + at] = (uint8_t)c;
-        tv[(d + 1) * UNIT + at] = (uint8_t)(c >> 8);
-      }
+    }
+    *(uint4 *)at = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  if (few) return;
-  __syncthreads();
-  const int low = grown_k ? b0 * s.block : from;
-  for (int i = tid + low * DP / 16; i < to * DP / 16; i += THREADS) ((uint4 *)gk)[i] = ((const uint4 *)lk)[i];
-  for (int i = tid; i < VP * UNIT / 16; i += THREADS) ((uint4 *)gv)[i] = ((const uint4 *)lv)[i];
 }
 
-// bf16 of a code times a power of two: exact where the result is a bf16 number
-__device__ __forceinline__ uint16_t value(uint32_t code, float scale) { return kx_bf16_rne(__builtin_amdgcn_cvt_f32_fp8((int)code, 0) * scale); }
+// eight codes times a power of two as bf16, which holds them exactly, at element d of a row of n; wide: rows and d are whole pieces of 16 bytes
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+template <bool HIGH>
+__device__ __forceinline__ uint32_t values(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, scale, HIGH));
+}
+__device__ __forceinline__ void put(uint16_t *row, int d, int n, bool wide, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  if (wide) {
+    if (d < n) *(uint4 *)(row + d) = make_uint4(x, y, z, w);
+    return;
+  }
+  const uint32_t v[4] = {x, y, z, w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (d + e < n) row[d + e] = (uint16_t)(v[e >> 1] >> 16 * (e & 1));
+}
 
 template <int DP, int VP>
 __global__ void __launch_bounds__(THREADS) read_k(KxPagedArgs a) {
-  __shared__ __attribute__((aligned(16))) uint8_t lv[VP * UNIT];
   const KxPagedSpec &s = a.s;
-  const Unit u = unit_of(a);
-  if (!u.ok) return;
+  Unit u = unit_of(a);
+  if (!u.to || !placed(a, u)) return;
   const int tid = threadIdx.x;
   const uint8_t *const gk = a.k + (u.head * s.page + u.in_page) * DP, *const gv = a.v + (u.head * s.page + u.in_page) * VP;
-  const size_t sc = u.head * (s.page / s.block) + u.in_page / s.block;
+  const size_t sc = u.head * (s.page >> a.block_bits) + (u.in_page >> a.block_bits);
   uint16_t *const ok = (uint16_t *)a.out + (size_t)u.row * a.out_ld + (size_t)blockIdx.y * s.dim;
   uint16_t *const ov = (uint16_t *)a.out_v + (size_t)u.row * a.out_v_ld + (size_t)blockIdx.y * s.vdim;
-  for (int i = tid; i < VP * UNIT / 16; i += THREADS) ((uint4 *)lv)[i] = ((const uint4 *)gv)[i];
-  for (int i = tid; i < (u.to - u.from) * (DP / 2); i += THREADS) {
-    const int t = u.from + i / (DP / 2), d = i % (DP / 2) * 2;
-    const uint32_t c = *(const uint16_t *)(gk + t * DP + d);
-    const float f = a.ks[sc + t / s.block];
-    uint16_t *const to = ok + (size_t)(t - u.from) * a.out_ld + d;
-    if (d < s.dim) to[0] = value(c, f);
-    if (d + 1 < s.dim) to[1] = value(c >> 8, f);
+  for (int i = tid; i < VP / 8 * 16; i += THREADS) {  // eight words of 8 rows by eight of them a wave: whole lines of results
+    const int word = (i & 7) | (i >> 6 & 1) << 3, d = ((i >> 3 & 7) | i >> 7 << 3) * 8, t = token_of(word * 4);
+    if (t + 3 < u.from || t >= u.to) continue;
+    uint32_t w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = *(const uint32_t *)(gv + (d + e) * UNIT + word * 4);
+    const float f = a.vs[sc + (t >> a.block_bits)];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // tokens t + 2 h and t + 2 h + 1
+      uint32_t c[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], h ? 0x07030602u : 0x05010400u);
+      const int at = t + 2 * h;
+      if (at >= u.from && at < u.to)
+        put(ov + (size_t)(at - u.from) * a.out_v_ld, d, s.vdim, a.wide_v, values<false>(c[0], f), values<false>(c[1], f), values<false>(c[2], f), values<false>(c[3], f));
+      if (at + 1 >= u.from && at + 1 < u.to)
+        put(ov + (size_t)(at + 1 - u.from) * a.out_v_ld, d, s.vdim, a.wide_v, values<true>(c[0], f), values<true>(c[1], f), values<true>(c[2], f), values<true>(c[3], f));
+    }
   }
-  __syncthreads();
-  for (int i = tid; i < (u.to - u.from) * VP; i += THREADS) {
-    const int t = u.from + i / VP, d = i % VP;
-    if (d < s.vdim) ov[(size_t)(t - u.from) * a.out_v_ld + d] = value(lv[d * UNIT + place_of(t)], a.vs[sc + t / s.block]);
+  for (int i = tid; i < (u.to - u.from) * (DP / 8); i += THREADS) {
+    const int t = u.from + i / (DP / 8), d = i % (DP / 8) * 8;
+    const uint2 c = *(const uint2 *)(gk + t * DP + d);
+    const float f = a.ks[sc + (t >> a.block_bits)];
+    put(ok + (size_t)(t - u.from) * a.out_ld, d, s.dim, a.wide_k, values<false>(c.x, f), values<true>(c.x, f), values<false>(c.y, f), values<true>(c.y, f));
   }
 }
 
@@ -278,8 +331,8 @@ int by_widths(const KxPagedSpec &s, F f) {
   KX_LAUNCH_CHECK();
   return KX_OK;
 }
-// groups of 64 that so many rows of so many sequences can lie in: n of a sequence in at most 2 + (n - 2) / 64
-unsigned most_units(const KxPagedArgs &a) { return (unsigned)(2 * std::min(a.batch, a.tokens) + a.tokens / UNIT); }
+// groups of 64 that so many rows of so many sequences can lie in: n of a sequence in at most n, and in at most 2 + (n - 2) / 64
+unsigned most_units(const KxPagedArgs &a) { return (unsigned)std::min(a.tokens, 2 * std::min(a.batch, a.tokens) + a.tokens / UNIT); }
 
 }  // namespace
 
@@ -399,6 +452,8 @@ extern "C" int kx_paged_read(kx_paged *p, const kx_paged_cache *cache, const kx_
   KX_REQUIRE(d_k && d_v && (uintptr_t)d_k % 2 == 0 && (uintptr_t)d_v % 2 == 0 && k_ld >= a.s.kv_heads * a.s.dim && v_ld >= a.s.kv_heads * a.s.vdim, "kx_paged_read: k_ld=%d v_ld=%d", k_ld, v_ld);
   if (!a.tokens) return KX_OK;
   a.out = d_k; a.out_ld = k_ld; a.out_v = d_v; a.out_v_ld = v_ld;
+  a.wide_k = (uintptr_t)d_k % 16 == 0 && k_ld % 8 == 0 && a.s.dim % 8 == 0;
+  a.wide_v = (uintptr_t)d_v % 16 == 0 && v_ld % 8 == 0 && a.s.vdim % 8 == 0;
   return kx_paged_read_launch(a, kx_stream(stream));
 }
 extern "C" int kx_paged_attend(kx_paged *p, const kx_paged_cache *cache, const kx_paged_rows *rows, const void *d_proj, int32_t proj_ld, int32_t q_off, void *d_out, int32_t out_ld, void *stream) {
