@@ -1,11 +1,11 @@
 // kx_paged_cache.hip -- keys and values into the pages of an 8-bit cache and out of them again (kx_paged.h).  No counterpart in the reference,
 // which stores 32-bit keys and values tile by tile on a disk (KvCache, src/kimi_exec.cu:192-238).
 //
-// append: a workgroup has the new tokens that lie in one group of 64 of a sequence, for one head of keys and values, and wave w of its four the tokens whose
-//   values are bytes 16 w .. 16 w + 15 of a row: 16 j + 4 w + r.  Every element is read once, turned by its position in 64 bits -- three sines and cosines a
-//   lane, the others by addition of angles -- and kept as a float whose last bit says whether anything was cut off; rounding that to 4 bits of fraction at any
-//   scale is one rounding of the exact number.  The largest magnitude of each block goes through LDS; with the scales known, codes are made in registers and
-//   go straight to the pages: keys a row at a time, values 16 bytes of a row at a time, with the older ones of those 16 where there are any.
+// append: a workgroup has the new tokens that lie in one group of 64 of a sequence, for one head of keys and values, and each of its four waves 16 tokens in
+//   a row.  Every element is read once, turned by its position in 64 bits -- two sines and cosines a lane, the others by addition of angles -- and kept as a
+//   float that any rounding to 4 bits of fraction takes where it takes the exact number.  The largest magnitude of each block goes through LDS; with the
+//   scales known, codes are made in registers and put together in LDS: whole rows of keys, and pieces of 16 bytes of the values, with the older ones of
+//   those 16 where there are any.
 // read: the same groups, codes times scales as bf16, which holds them exactly; values are turned four tokens by eight dimensions a lane.
 #include <algorithm>
 #include <cmath>
@@ -23,24 +23,24 @@ using namespace kxpage;
 
 constexpr int THREADS = 256, FEW = 4;  // FEW: most tokens whose values are stored byte by byte
 
-// x with its last bits cut off, and the last that is left set where that changed anything; less than any code can hold becomes zero
-__device__ __forceinline__ float sticky(double x) {
-  const uint64_t u = (uint64_t)__double_as_longlong(x);
-  const uint32_t hi = (uint32_t)(u >> 32), size = hi & 0x7fffffffu;
-  uint32_t f = (uint32_t)(u >> 29) - (896u << 23) | ((uint32_t)u & 0x1fffffffu ? 1u : 0u);
-  f = size < 897u << 20 ? 0u : size >= 1151u << 20 ? 0x7f7fffffu : f & 0x7fffffffu;
-  f = size >= 0x7ff00000u ? 0x7fc00000u : f;
-  return kx_bits_f32(f | (hi & 0x80000000u));
+// Two numbers as floats that round to 4 bits of fraction, and lie next to a power of two times 1.75, as they do themselves: a float on a border between two
+// codes has 19 zeros at its end, and only then its last bit is set where the number is not the float.
+__device__ __forceinline__ float off_border(float f, double x) {
+  const uint32_t u = kx_f32_bits(f);
+  if (u & 0x7ffffu || (double)f == x || f != f) return f;
+  return kx_bits_f32(__builtin_fabs((double)f) > __builtin_fabs(x) ? u - 1 : u | 1);
 }
-__device__ __forceinline__ uint32_t magnitude(float x) {  // bits of |x|; 0 for what is not finite
-  const uint32_t u = kx_f32_bits(x) & 0x7fffffffu;
-  return u >= 0x7f800000u ? 0u : u;
+__device__ __forceinline__ void rounded(double x, double y, float &a, float &b) {
+  a = (float)x;
+  b = (float)y;
+  if (__builtin_amdgcn_ballot_w64((kx_f32_bits(a) & 0x7ffffu) == 0 || (kx_f32_bits(b) & 0x7ffffu) == 0)) {
+    a = off_border(a, x);
+    b = off_border(b, y);
+  }
 }
-// codes of two numbers at the scale whose reciprocal is given, in the low 16 bits
-__device__ __forceinline__ uint32_t codes(float a, float b, float inverse) {
-  auto scaled = [&](float x) { return (kx_f32_bits(x) & 0x7f800000u) == 0x7f800000u ? __builtin_nanf("") : x * inverse; };
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(scaled(a), scaled(b), 0, false) & 0xffffu;
-}
+__device__ __forceinline__ float finite(float x) { return __builtin_fabsf(x) < __builtin_inff() ? x : 0.0f; }  // largest magnitudes leave out what is not
+// codes of two numbers of at most 448, in the low 16 bits; NaN of what is not finite
+__device__ __forceinline__ uint32_t codes(float a, float b) { return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu; }
 // the four codes of a word divided by 2^down
 __device__ __forceinline__ uint32_t lowered(uint32_t w, int down) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -84,187 +84,158 @@ __device__ __forceinline__ uint32_t bytes_within(int t, int from, int to) {
 
 template <int DP, int VP>
 __global__ void __launch_bounds__(THREADS) append_k(KxPagedArgs a) {
-  constexpr int PK = (DP + 127) / 128, PV = VP / 64;  // of a lane: pairs of a key, elements of a value
-  __shared__ uint32_t most[4][8];
+  constexpr int PK = (DP + 127) / 128, PV = VP / 64, NW = THREADS / 64, MINE = UNIT / NW;  // of a lane: pairs of a key, elements of a value; tokens of a wave
+  constexpr int LD = UNIT + 16;                                                            // bytes of a row of values in LDS
+  __shared__ __attribute__((aligned(16))) uint8_t lk[UNIT * DP], lv[VP * LD];
+  __shared__ float most[2][NW];
   const KxPagedSpec &s = a.s;
   Unit u = unit_of(a);
   if (!u.to) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), from = u.from, to = u.to, t0 = 4 * wave;
-  auto fresh = [&](int j, int r) { return t0 + 16 * j + r >= from && t0 + 16 * j + r < to; };
-  float xk[4][4][PK][2], xv[4][4][PV];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), from = u.from, to = u.to, t0 = MINE * wave;
+  const int mine_from = max(from - t0, 0), mine_to = min(to - t0, MINE);  // the wave's new tokens
+  float xk[MINE][PK][2], xv[MINE][PV];
   double turn[PK];
 #pragma unroll
   for (int p = 0; p < PK; ++p) turn[p] = lane + 64 * p < s.rot / 2 ? a.turn[lane + 64 * p] : 0.0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int i = 0; i < MINE; ++i) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int p = 0; p < PK; ++p) xk[i][p][0] = xk[i][p][1] = 0.0f;
 #pragma unroll
-      for (int p = 0; p < PK; ++p) xk[j][r][p][0] = xk[j][r][p][1] = 0.0f;
+    for (int p = 0; p < PV; ++p) xv[i][p] = 0.0f;
+    if (i < mine_from || i >= mine_to) continue;
+    const float *const row = a.proj + (size_t)(u.row + t0 + i - from) * a.proj_ld;
+    const float *const rk = row + a.k_off + (size_t)blockIdx.y * s.dim, *const rv = row + a.v_off + (size_t)blockIdx.y * s.vdim;
 #pragma unroll
-      for (int p = 0; p < PV; ++p) xv[j][r][p] = 0.0f;
-      if (!fresh(j, r)) continue;
-      const float *const row = a.proj + (size_t)(u.row + t0 + 16 * j + r - from) * a.proj_ld;
-      const float *const rk = row + a.k_off + (size_t)blockIdx.y * s.dim, *const rv = row + a.v_off + (size_t)blockIdx.y * s.vdim;
-#pragma unroll
-      for (int p = 0; p < PK; ++p) {
-        const int2 d = pair_of(lane + 64 * p, s.rot, s.pairs);
-        if (d.x < s.dim) xk[j][r][p][0] = rk[d.x];
-        if (d.y < s.dim) xk[j][r][p][1] = rk[d.y];
-      }
-#pragma unroll
-      for (int p = 0; p < PV; ++p)
-        if (lane + 64 * p < s.vdim) xv[j][r][p] = rv[lane + 64 * p];
+    for (int p = 0; p < PK; ++p) {
+      const int2 d = pair_of(lane + 64 * p, s.rot, s.pairs);
+      if (d.x < s.dim) xk[i][p][0] = rk[d.x];
+      if (d.y < s.dim) xk[i][p][1] = rk[d.y];
     }
+#pragma unroll
+    for (int p = 0; p < PV; ++p)
+      if (lane + 64 * p < s.vdim) xv[i][p] = rv[lane + 64 * p];
+  }
   if (!placed(a, u)) return;
   uint8_t *const gk = a.k + (u.head * s.page + u.in_page) * DP, *const gv = a.v + (u.head * s.page + u.in_page) * VP;
   const size_t sc = u.head * (s.page >> a.block_bits) + (u.in_page >> a.block_bits);  // scale of the group's first block
-  const int b0 = from >> a.block_bits, per = s.block / 16;
+  const int b0 = from >> a.block_bits;
   const bool kept = (from & (s.block - 1)) != 0;  // the first block has older tokens
   const int old_k = kept ? scale_exponent(kx_f32_bits(a.ks[sc + b0])) : 0, old_v = kept ? scale_exponent(kx_f32_bits(a.vs[sc + b0])) : 0;
 
-  // turns: of the wave's first four tokens with new ones among them, of one token, of 16
-  const bool single = to - from == 1;
-  const int j0 = (from - t0 + 12) >> 4;
-  double c0[PK], s0[PK], c1[PK], s1[PK], c16[PK], s16[PK];
-#pragma unroll
-  for (int p = 0; p < PK; ++p) {
-    auto eval = [&](int n, double &c, double &s) {
-      const double at = turn[p] * (double)n;
-      turned(at - __builtin_rint(at), c, s);
-    };
-    c1[p] = c16[p] = 1.0;
-    s1[p] = s16[p] = 0.0;
-    eval(u.pos + (single ? from : t0 + 16 * j0), c0[p], s0[p]);
-    if (!single) eval(1, c1[p], s1[p]);
-    if (to - from > 4) eval(16, c16[p], s16[p]);
-  }
-  uint32_t mk[4] = {0, 0, 0, 0}, mv[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j < j0 || t0 + 16 * j >= to) continue;
+  float mk = 0.0f, mv = 0.0f;
+  if (mine_from < mine_to) {
 #pragma unroll
     for (int p = 0; p < PK; ++p) {
-      double c = c0[p], n = s0[p];
+      auto eval = [&](int n, double &c, double &s) {
+        const double at = turn[p] * (double)n;
+        turned(at - __builtin_rint(at), c, s);
+      };
+      double c, n, c1 = 1.0, n1 = 0.0;
+      eval(u.pos + t0 + mine_from, c, n);
+      if (mine_to - mine_from > 1) eval(1, c1, n1);
+      const bool turns = lane + 64 * p < s.rot / 2;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (fresh(j, r)) {
-          float &x = xk[j][r][p][0], &y = xk[j][r][p][1];
-          if (lane + 64 * p < s.rot / 2) {
-            const double x0 = x, y0 = y;
-            x = sticky(x0 * c - y0 * n);
-            y = sticky(x0 * n + y0 * c);
-          }
-          mk[j] = max(mk[j], max(magnitude(x), magnitude(y)));
-        }
-        if (r < 3 && !single) {
-          const double d = c * c1[p] - n * s1[p];
-          n = c * s1[p] + n * c1[p];
-          c = d;
-        }
+      for (int i = 0; i < MINE; ++i) {
+        if (i < mine_from || i >= mine_to) continue;
+        float &x = xk[i][p][0], &y = xk[i][p][1];
+        if (turns) rounded(__builtin_fma(-(double)y, n, x * c), __builtin_fma((double)y, c, x * n), x, y);
+        mk = fmaxf(mk, fmaxf(__builtin_fabsf(x), __builtin_fabsf(y)));
+        const double d = __builtin_fma(-n, n1, c * c1);
+        n = __builtin_fma(n, c1, c * n1);
+        c = d;
       }
-      const double d = c0[p] * c16[p] - s0[p] * s16[p];
-      s0[p] = c0[p] * s16[p] + s0[p] * c16[p];
-      c0[p] = d;
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int i = 0; i < MINE; ++i)
 #pragma unroll
-      for (int p = 0; p < PV; ++p) mv[j] = max(mv[j], magnitude(xv[j][r][p]));
-    mk[j] = kx_f32_bits(kxw::wave_max_f32(kx_bits_f32(mk[j])));
-    mv[j] = kx_f32_bits(kxw::wave_max_f32(kx_bits_f32(mv[j])));
+      for (int p = 0; p < PV; ++p) mv = fmaxf(mv, __builtin_fabsf(xv[i][p]));
+    mk = kxw::wave_max_f32(mk);
+    mv = kxw::wave_max_f32(mv);
+    if (!(fmaxf(mk, mv) < __builtin_inff())) {
+      mk = mv = 0.0f;
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+#pragma unroll
+        for (int p = 0; p < PK; ++p) mk = fmaxf(mk, fmaxf(__builtin_fabsf(finite(xk[i][p][0])), __builtin_fabsf(finite(xk[i][p][1]))));
+#pragma unroll
+        for (int p = 0; p < PV; ++p) mv = fmaxf(mv, __builtin_fabsf(finite(xv[i][p])));
+      }
+      mk = kxw::wave_max_f32(mk);
+      mv = kxw::wave_max_f32(mv);
+    }
   }
   if (lane == 0) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      most[wave][j] = mk[j];
-      most[wave][4 + j] = mv[j];
-    }
+    most[0][wave] = mk;
+    most[1][wave] = mv;
   }
   __syncthreads();
-  // exponents of the blocks that the group's four blocks of 16 lie in
-  int ek[4], ev[4];
+  // exponents of block b, before and with the new tokens
+  const int bits = a.block_bits, per = s.block / MINE;
+  auto exponent = [&](int which, int b, int old) {
+    float m = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    mk[j] = max(max(most[0][j], most[1][j]), max(most[2][j], most[3][j]));
-    mv[j] = max(max(most[0][4 + j], most[1][4 + j]), max(most[2][4 + j], most[3][4 + j]));
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t k2 = max(mk[j & 2], mk[j | 1]), v2 = max(mv[j & 2], mv[j | 1]), k4 = max(max(mk[0], mk[1]), max(mk[2], mk[3])), v4 = max(max(mv[0], mv[1]), max(mv[2], mv[3]));
-    ek[j] = exponent_of(per == 1 ? mk[j] : per == 2 ? k2 : k4);
-    ev[j] = exponent_of(per == 1 ? mv[j] : per == 2 ? v2 : v4);
-    if (kept && j / per == b0) {
-      ek[j] = max(ek[j], old_k);
-      ev[j] = max(ev[j], old_v);
-    }
-  }
-  // the exponents of the first block that the group writes to
-  const int g0 = b0 * per, ek0 = g0 == 0 ? ek[0] : g0 == 1 ? ek[1] : g0 == 2 ? ek[2] : ek[3], ev0 = g0 == 0 ? ev[0] : g0 == 1 ? ev[1] : g0 == 2 ? ev[2] : ev[3];
-  const int grown_k = kept ? ek0 - old_k : 0, grown_v = kept ? ev0 - old_v : 0;
-  if (tid < 4 && (tid & (per - 1)) == 0 && tid / per >= b0 && tid / per <= (to - 1) >> a.block_bits) {
-    const int k = tid == 0 ? ek[0] : tid == 1 ? ek[1] : tid == 2 ? ek[2] : ek[3], v = tid == 0 ? ev[0] : tid == 1 ? ev[1] : tid == 2 ? ev[2] : ev[3];
-    a.ks[sc + tid / per] = kx_bits_f32(scale_bits(k));
-    a.vs[sc + tid / per] = kx_bits_f32(scale_bits(v));
+    for (int w = 0; w < NW; ++w) m = w / per == b ? fmaxf(m, most[which][w]) : m;
+    const int e = exponent_of(kx_f32_bits(m));
+    return kept && b == b0 ? max(e, old) : e;
+  };
+  const int b = t0 >> bits, ek = exponent(0, b, old_k), ev = exponent(1, b, old_v);
+  const int grown_k = kept ? exponent(0, b0, old_k) - old_k : 0, grown_v = kept ? exponent(1, b0, old_v) - old_v : 0;
+  if (lane == 0 && (t0 & (s.block - 1)) == 0 && b >= b0 && b <= (to - 1) >> bits) {
+    a.ks[sc + b] = kx_bits_f32(scale_bits(ek));
+    a.vs[sc + b] = kx_bits_f32(scale_bits(ev));
   }
 
-  // keys
   if (grown_k) {
     uint32_t *const w = (uint32_t *)(gk + b0 * s.block * DP);
     for (int i = tid; i < (from - b0 * s.block) * (DP / 4); i += THREADS) w[i] = lowered(w[i], grown_k);
   }
+  const float rk = kx_bits_f32(scale_bits(-ek)), rv = kx_bits_f32(scale_bits(-ev));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float rk = kx_bits_f32(scale_bits(-ek[j]));
+  for (int i = 0; i < MINE; ++i) {
+    if (i < mine_from || i >= mine_to) continue;
+    uint8_t *const row = lk + (t0 + i) * DP;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (!fresh(j, r)) continue;
-      uint8_t *const row = gk + (t0 + 16 * j + r) * DP;
-#pragma unroll
-      for (int p = 0; p < PK; ++p)
-        if (lane + 64 * p < DP / 2) {
-          const int2 d = pair_of(lane + 64 * p, s.rot, s.pairs);
-          const uint32_t c = codes(xk[j][r][p][0], xk[j][r][p][1], rk);
-          if (d.y == d.x + 1) {
-            *(uint16_t *)(row + d.x) = (uint16_t)c;
-          } else {
-            row[d.x] = (uint8_t)c;
-            row[d.y] = (uint8_t)(c >> 8);
-          }
-        }
-    }
+    for (int p = 0; p < PK; ++p)
+      if (lane + 64 * p < DP / 2) {
+        const int2 d = pair_of(lane + 64 * p, s.rot, s.pairs);
+        const uint32_t c = codes(xk[i][p][0] * rk, xk[i][p][1] * rk);
+        row[d.x] = (uint8_t)c;
+        row[d.y] = (uint8_t)(c >> 8);
+      }
   }
-  // values
-  const bool any = j0 < 4 && t0 + 16 * j0 < to;
-  if (!any && !grown_v) return;
-  const bool few = to - from <= FEW && !grown_v, alone = from == 0 || (from <= t0 && to >= t0 + 52);
+  const bool few = to - from <= FEW && !grown_v;
 #pragma unroll
-  for (int p = 0; p < PV; ++p) {
-    uint8_t *const at = gv + (lane + 64 * p) * UNIT + 16 * wave;
-    uint32_t w[4];
+  for (int p = 0; p < PV; ++p)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float rv = kx_bits_f32(scale_bits(-ev[j]));
-      w[j] = codes(xv[j][0][p], xv[j][1][p], rv) | codes(xv[j][2][p], xv[j][3][p], rv) << 16;
-    }
-    if (few) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
+    for (int i = 0; i < MINE; i += 4) {
+      const uint32_t w = codes(xv[i][p] * rv, xv[i + 1][p] * rv) | codes(xv[i + 2][p] * rv, xv[i + 3][p] * rv) << 16;
+      const int d = lane + 64 * p, at = place_of(t0 + i);
+      if (!few) {
+        *(uint32_t *)(lv + d * LD + at) = w;
+      } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (fresh(j, r)) at[4 * j + r] = (uint8_t)(w[j] >> 8 * r);
-      continue;
-    }
-    if (!alone) {
-      const uint4 o = *(const uint4 *)at;
-      const uint32_t old[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t mask = bytes_within(t0 + 16 * j, from, to);
-        w[j] = (w[j] & mask) | ((grown_v && j / per == b0 ? lowered(old[j], grown_v) : old[j]) & ~mask);
+          if (i + r >= mine_from && i + r < mine_to) gv[d * UNIT + at + r] = (uint8_t)(w >> 8 * r);
       }
     }
-    *(uint4 *)at = make_uint4(w[0], w[1], w[2], w[3]);
+  __syncthreads();
+  for (int i = from * (DP / 16) + tid; i < to * (DP / 16); i += THREADS) ((uint4 *)gk)[i] = ((const uint4 *)lk)[i];
+  if (few) return;
+  for (int i = tid; i < VP * 4; i += THREADS) {  // 16 bytes: tokens 16 j + 4 q + 0 .. 3
+    const int q = i & 3;
+    uint4 *const at = (uint4 *)gv + i;
+    uint4 w = *(const uint4 *)(lv + (i >> 2) * LD + q * 16);
+    if (from > 0 && (from > 4 * q || to < 4 * q + 52)) {
+      if (!grown_v && (from > 4 * q + 51 || to <= 4 * q)) continue;
+      const uint4 old = *at;
+      auto mixed = [&](uint32_t n, uint32_t o, int j) {
+        const uint32_t mask = bytes_within(16 * j + 4 * q, from, to);
+        return (n & mask) | ((grown_v && 16 * j >> bits == b0 ? lowered(o, grown_v) : o) & ~mask);
+      };
+      w = make_uint4(mixed(w.x, old.x, 0), mixed(w.y, old.y, 1), mixed(w.z, old.z, 2), mixed(w.w, old.w, 3));
+    }
+    *at = w;
   }
 }
 
