@@ -71,7 +71,7 @@ struct Form {
   static constexpr int WAVES = REGISTERS > 200 ? 1 : 2;                         // per SIMD
   static constexpr int SUB = NQ == 1 ? 4 : 2;                                   // blocks of 16 tokens that are multiplied at a time
   static constexpr int QLD = DP + 4, OLD = 68;                                  // floats of a row in LDS: a query; 64 sums of a column
-  static constexpr int Q_FLOATS = (SHARE ? 1 : NW) * 16 * QLD, O_FLOATS = NW * 16 * OLD + 2 * NW * TILE;
+  static constexpr int Q_FLOATS = (SHARE ? TILE : NW * 16) * QLD, O_FLOATS = NW * 16 * OLD + 2 * NW * TILE;
   static constexpr int LDS = Q_FLOATS > O_FLOATS ? Q_FLOATS : O_FLOATS;
 };
 
@@ -104,10 +104,11 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
     lo[n] = low(hi[n]);
   }
 
-  // queries: asked for first, a wave a column and a lane a pair of dimensions; turned by their positions into LDS, 16 columns at a time, and from there to the lanes
-  // in the order of the keys' loads
-  constexpr int PP = (DP / 2 + 63) / 64, MINE = SHARE ? 16 / NW : 16;  // pairs of a lane; columns of a wave among 16
-  auto column = [&](int n, int k) { return min(c0 + n * 16 + (SHARE ? k * NW + wave : k), R - 1); };
+  // queries: asked for first, a wave a column and a lane a pair of dimensions; turned by their positions into LDS, and from there to the lanes in the order of the
+  // keys' loads.  All columns at once where the waves share them, 16 at a time where each has its own.
+  constexpr int PP = (DP / 2 + 63) / 64, MINE = SHARE ? TILE / NW : 16, NTH = SHARE ? NW : 1;  // pairs of a lane; a wave's columns at a time, every NTH
+  const int q_first = SHARE ? wave : 0;
+  auto column = [&](int n, int k) { return min(c0 + n * 16 + k * NTH + q_first, R - 1); };
   float qx[MINE][PP][2];
   auto ask_queries = [&](int n) {
 #pragma unroll
@@ -174,15 +175,15 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
 
   h8 q[NQ][DP / 32], ql[F32 ? NQ : 1][F32 ? DP / 32 : 1];
   float qf[NQ];
+  float *const rows = lds + (SHARE ? 0 : wave * 16 * FM::QLD);
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    float *const rows = lds + (SHARE ? 0 : wave * 16 * FM::QLD);
-    if (n) ask_queries(n);
+  for (int n0 = 0; n0 < NQ; n0 += SHARE ? NQ : 1) {
+    if (n0) ask_queries(n0);
     int turned_at = -1;
     float cs[PP], sn[PP];
 #pragma unroll
     for (int k = 0; k < MINE; ++k) {
-      const int at = row_of(column(n, k));
+      const int at = row_of(column(n0, k));
       if (at != turned_at) {
         turned_at = at;
 #pragma unroll
@@ -199,34 +200,37 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
         const int2 d = pair_of(lane + 64 * p, s.rot, s.pairs);
         const float u = qx[k][p][0], v = qx[k][p][1];
         const bool turns = lane + 64 * p < s.rot / 2;
-        float *const row = rows + (SHARE ? k * NW + wave : k) * FM::QLD;
+        float *const row = rows + (k * NTH + q_first) * FM::QLD;
         row[d.x] = turns ? u * cs[p] - v * sn[p] : u;
         row[d.y] = turns ? u * sn[p] + v * cs[p] : v;
       }
     }
     __syncthreads();
-    float most = 0.0f;
-    const float *const mine = rows + lc * FM::QLD + lq * 16;
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j)
+    for (int n = n0; n < (SHARE ? NQ : n0 + 1); ++n) {
+      float most = 0.0f;
+      const float *const mine = rows + ((n - n0) * 16 + lc) * FM::QLD + lq * 16;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float x = __builtin_fabsf(mine[j * 64 + e]);
-        most = fmaxf(most, x < __builtin_inff() ? x : 0.0f);
-      }
-    most = quarters_max(most);
-    const int e = max(min((int)(kx_f32_bits(most) >> 23) - 126, 120), -100);
-    const float down = kx_bits_f32(scale_bits(-e));
-    qf[n] = kx_bits_f32(scale_bits(e)) * s.scale * 1.44269504088896341f;
+      for (int j = 0; j < DP / 64; ++j)
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j)
+        for (int e = 0; e < 16; ++e) {
+          const float x = __builtin_fabsf(mine[j * 64 + e]);
+          most = fmaxf(most, x < __builtin_inff() ? x : 0.0f);
+        }
+      most = quarters_max(most);
+      const int e = max(min((int)(kx_f32_bits(most) >> 23) - 126, 120), -100);
+      const float down = kx_bits_f32(scale_bits(-e));
+      qf[n] = kx_bits_f32(scale_bits(e)) * s.scale * 1.44269504088896341f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float x = mine[j * 64 + e] * down;
-        const _Float16 h = (_Float16)x;
-        q[n][2 * j + (e >> 3)][e & 7] = h;
-        if constexpr (F32) ql[n][2 * j + (e >> 3)][e & 7] = (_Float16)(x - (float)h);
-      }
+      for (int j = 0; j < DP / 64; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = mine[j * 64 + e] * down;
+          const _Float16 h = (_Float16)x;
+          q[n][2 * j + (e >> 3)][e & 7] = h;
+          if constexpr (F32) ql[n][2 * j + (e >> 3)][e & 7] = (_Float16)(x - (float)h);
+        }
+    }
     __syncthreads();
   }
 
@@ -481,52 +485,82 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
   __syncthreads();
   if (!last) return;
   if (threadIdx.x == 0) kx_arrive_reset(arrived);
-  // weights of the parts, a wave a column and a lane a part; then their sums
+  // sums of the parts: a lane four dimensions of ITEMS columns, AT_ONCE parts at a time; the first of them are asked for before the weights are worked out, 16
+  // lanes a column
   const int cols = min(COLS, R - w0);
   float2 *const st = (float2 *)lds;  // [used][COLS]
-  for (int i = threadIdx.x; i < used * COLS; i += FM::THREADS)
-    if (i % COLS < cols) {
-      const uint64_t w = kx_arrive_load((const uint64_t *)(part + (size_t)(i / COLS) * FM::PART + (size_t)COLS * VP) + i % COLS);
-      st[i] = make_float2(kx_bits_f32((uint32_t)w), kx_bits_f32((uint32_t)(w >> 32)));
+  auto stat_of = [&](int i) { return kx_arrive_load((const uint64_t *)(part + (size_t)(i / COLS) * FM::PART + (size_t)COLS * VP) + i % COLS); };
+  auto keep = [&](int i, uint64_t w) { st[i] = make_float2(kx_bits_f32((uint32_t)w), kx_bits_f32((uint32_t)(w >> 32))); };
+  const bool first_stat = (int)threadIdx.x < used * COLS && (int)threadIdx.x % COLS < cols;
+  const uint64_t first_word = first_stat ? stat_of(threadIdx.x) : 0;
+  auto weights = [&]() {
+    if (first_stat) keep(threadIdx.x, first_word);
+    for (int i = threadIdx.x + FM::THREADS; i < used * COLS; i += FM::THREADS)
+      if (i % COLS < cols) keep(i, stat_of(i));
+    __syncthreads();
+    for (int c = threadIdx.x >> 4; c < cols; c += FM::THREADS / 16) {
+      float most = NONE, sum = 0.0f;
+      for (int p = lc; p < used; p += 16) most = fmaxf(most, st[p * COLS + c].x);
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+      for (int p = lc; p < used; p += 16) sum = __builtin_fmaf(st[p * COLS + c].y, exp2_(st[p * COLS + c].x - most), sum);
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d);
+      const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+      for (int p = lc; p < used; p += 16) st[p * COLS + c].x = exp2_(st[p * COLS + c].x - most) * f;
     }
-  __syncthreads();
-  for (int c = wave; c < cols; c += NW) {
-    float most = NONE, sum = 0.0f;
-    for (int p = lane; p < used; p += 64) most = fmaxf(most, st[p * COLS + c].x);
-    most = kxw::wave_max_f32(most);
-    for (int p = lane; p < used; p += 64) sum = __builtin_fmaf(st[p * COLS + c].y, exp2_(st[p * COLS + c].x - most), sum);
+    __syncthreads();
+  };
+  auto add_up = [&](auto items_, auto at_once_) {
+    constexpr int ITEMS = items_(), AT_ONCE = at_once_();
+    const int items = cols * (VP / 4);
+    bool weighed = false;
+    for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < items; i0 += ITEMS * FM::THREADS) {
+      f4 y[ITEMS];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-    for (int p = lane; p < used; p += 64) st[p * COLS + c].x = exp2_(st[p * COLS + c].x - most) * f;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < cols * (VP / 4); i += FM::THREADS) {
-    const int c = i / (VP / 4), d = i % (VP / 4) * 4;
-    const uint64_t *from = (const uint64_t *)(part + (size_t)c * VP + d);
-    f4 y = {0, 0, 0, 0};
-    constexpr int AT_ONCE = 16;
-    for (int p0 = 0; p0 < used; p0 += AT_ONCE) {
-      uint64_t w[AT_ONCE][2];
+      for (int n = 0; n < ITEMS; ++n) y[n] = f4{0, 0, 0, 0};
+      for (int p0 = 0; p0 < used; p0 += AT_ONCE) {
+        uint64_t w[ITEMS][AT_ONCE][2];
 #pragma unroll
-      for (int k = 0; k < AT_ONCE; ++k)
-        if (p0 + k < used) {
-          const size_t at = (size_t)(p0 + k) * (FM::PART / 2);
-          w[k][0] = kx_arrive_load(from + at);
-          w[k][1] = kx_arrive_load(from + at + 1);
+        for (int n = 0; n < ITEMS; ++n) {
+          const uint64_t *const from = (const uint64_t *)(part + (size_t)min(i0 + n * FM::THREADS, items - 1) * 4);
+#pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k)
+            if (p0 + k < used) {
+              const size_t at = (size_t)(p0 + k) * (FM::PART / 2);
+              w[n][k][0] = kx_arrive_load(from + at);
+              w[n][k][1] = kx_arrive_load(from + at + 1);
+            }
+        }
+        if (!weighed) {
+          weights();
+          weighed = true;
         }
 #pragma unroll
-      for (int k = 0; k < AT_ONCE; ++k) {
-        if (p0 + k >= used) continue;
-        const float f = st[(p0 + k) * COLS + c].x;
-        y[0] = __builtin_fmaf(kx_bits_f32((uint32_t)w[k][0]), f, y[0]);
-        y[1] = __builtin_fmaf(kx_bits_f32((uint32_t)(w[k][0] >> 32)), f, y[1]);
-        y[2] = __builtin_fmaf(kx_bits_f32((uint32_t)w[k][1]), f, y[2]);
-        y[3] = __builtin_fmaf(kx_bits_f32((uint32_t)(w[k][1] >> 32)), f, y[3]);
+        for (int n = 0; n < ITEMS; ++n) {
+          const int c = min((i0 + n * FM::THREADS) / (VP / 4), cols - 1);
+          float f[AT_ONCE];
+#pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k) f[k] = st[min(p0 + k, used - 1) * COLS + c].x;
+#pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k) {
+            if (p0 + k >= used) break;
+            y[n][0] = __builtin_fmaf(kx_bits_f32((uint32_t)w[n][k][0]), f[k], y[n][0]);
+            y[n][1] = __builtin_fmaf(kx_bits_f32((uint32_t)(w[n][k][0] >> 32)), f[k], y[n][1]);
+            y[n][2] = __builtin_fmaf(kx_bits_f32((uint32_t)w[n][k][1]), f[k], y[n][2]);
+            y[n][3] = __builtin_fmaf(kx_bits_f32((uint32_t)(w[n][k][1] >> 32)), f[k], y[n][3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < ITEMS; ++n) {
+        const int i = i0 + n * FM::THREADS;
+        if (i < items) give(w0 + i / (VP / 4), i % (VP / 4) * 4, y[n]);
       }
     }
-    give(w0 + c, d, y);
-  }
+  };
+  if (used <= 8) add_up(std::integral_constant<int, 2>(), std::integral_constant<int, 8>());
+  else add_up(std::integral_constant<int, 1>(), std::integral_constant<int, 16>());
 }
 
 template <class FM>
