@@ -17,6 +17,7 @@
 #include "kx_common.h"
 #include "kx_math.h"
 #include "kx_paged.h"
+#include "kx_read_once.h"
 #include "kx_wave.h"
 
 namespace {
@@ -61,10 +62,20 @@ __device__ __forceinline__ float quarters_sum(float v) {
 __device__ __forceinline__ h2 halves_of(float a, float b) { return __builtin_convertvector((f2{a, b}), h2); }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-template <int DP_, int VP_, int NQ_, bool SHARE_, bool F32_>
+template <bool ONCE>
+__device__ __forceinline__ uint4 piece(const uint8_t *p) {
+  if constexpr (ONCE) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const u4 w = __builtin_nontemporal_load((const u4 *)p);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return *(const uint4 *)p;
+}
+
+template <int DP_, int VP_, int NQ_, bool SHARE_, bool F32_, bool ONCE_ = false>
 struct Form {
   static constexpr int DP = DP_, VP = VP_, NQ = NQ_, NW = 4, THREADS = NW * 64, TILE = 16 * NQ;  // columns of a wave
-  static constexpr bool SHARE = SHARE_, F32 = F32_;
+  static constexpr bool SHARE = SHARE_, F32 = F32_, ONCE = ONCE_;
   static constexpr int COLS = SHARE ? TILE : NW * TILE;                         // of a workgroup
   static constexpr size_t PART = (size_t)COLS * (VP + 2);                       // floats of a part: sums, then M and denominator
   static constexpr int REGISTERS = NQ * (DP / 8 * (F32 ? 2 : 1) + VP / 4 + 16) + DP / 4 + VP / 4;
@@ -143,12 +154,12 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int j = 0; j < DP / 64; ++j) kr[tt][j] = *(const uint4 *)(k + tt * 16 * DP + j * 64);
+      for (int j = 0; j < DP / 64; ++j) kr[tt][j] = piece<FM::ONCE>(k + tt * 16 * DP + j * 64);
   };
   auto load_v = [&](int u, int id) {
     const uint8_t *const v = a.v + (head_of(id) * s.page + in_page(u)) * VP + lc * UNIT + lq * 16;
 #pragma unroll
-    for (int i = 0; i < VP / 16; ++i) vr[i] = *(const uint4 *)(v + i * 16 * UNIT);
+    for (int i = 0; i < VP / 16; ++i) vr[i] = piece<FM::ONCE>(v + i * 16 * UNIT);
   };
   // scales of the four blocks of 16 of a group
   auto load_scales = [&](int u, int id) {
@@ -590,6 +601,9 @@ int launch_columns(const KxPagedArgs &a, hipStream_t st) {
   const int g = a.s.heads / a.s.kv_heads;
   const long columns = (long)a.tokens * g / std::min(a.batch, a.tokens);  // of a sequence, on average
   constexpr int NQ = DP == 256 ? 1 : 2;  // the widest rows leave registers for one block of columns
+  // a cache that no level of caches holds is read past them where one workgroup reads each of its positions: 269 MB 62 -> 56 us, 640 MB 128 -> 124; with 131 MB,
+  // which the last level holds from one call to the next in a program of one layer, it takes 27 us instead of 24
+  if (columns <= 16 && kxonce::latent((size_t)std::min(a.batch, a.tokens) * a.longest * a.s.kv_heads * (DP + VP))) return launch<Form<DP, VP, 1, true, F32, true>>(a, g, st);
   if (columns <= 16) return launch<Form<DP, VP, 1, true, F32>>(a, g, st);
   if (columns <= 64) return launch<Form<DP, VP, NQ, true, F32>>(a, g, st);
   return launch<Form<DP, VP, NQ, false, F32>>(a, g, st);
