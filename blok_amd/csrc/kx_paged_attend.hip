@@ -230,8 +230,8 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
         }
       most = quarters_max(most);
       const int e = max(min((int)(kx_f32_bits(most) >> 23) - 126, 120), -100);
-      const float down = kx_bits_f32(scale_bits(-e));
-      qf[n] = kx_bits_f32(scale_bits(e)) * s.scale * 1.44269504088896341f;
+      const float down = s.scale == 0.0f ? 0.0f : __builtin_copysignf(kx_bits_f32(scale_bits(-e)), s.scale);
+      qf[n] = kx_bits_f32(scale_bits(e)) * __builtin_fabsf(s.scale) * 1.44269504088896341f;
 #pragma unroll
       for (int j = 0; j < DP / 64; ++j)
 #pragma unroll
@@ -319,12 +319,6 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
       h8 ph[NQ][SUB / 2], pl[F32 ? NQ : 1][SUB / 2];
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-        for (int tt = 0; tt < SUB; ++tt) {
-          const float f = qf[n] * kx_bits_f32(ks[t0 + tt]), e = (float)scale_exponent(vs[t0 + tt]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[n][tt][i] = __builtin_fmaf(x[n][tt][i], f, e);
-        }
         if (!whole) {
           // positions of the lane's tokens that its column sees, counted from its first token
           const int from = there ? lo[n] - (base + t0 * 16 + lq * 4) : 1 << 30, to = hi[n] - (base + t0 * 16 + lq * 4);
@@ -333,11 +327,14 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[n][tt][i] = ((tt * 16 + i > to) | (tt * 16 + i < from)) ? -__builtin_inff() : x[n][tt][i];
         }
-        float most = NONE;
+        // x = score f + b, which grows with the score: the largest of a block's by its largest score.  f is above zero, so that -inf stays
+        float most = NONE, f[SUB];
 #pragma unroll
-        for (int tt = 0; tt < SUB; ++tt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) most = fmaxf(most, x[n][tt][i]);
+        for (int tt = 0; tt < SUB; ++tt) {
+          f[tt] = fmaxf(qf[n] * kx_bits_f32(ks[t0 + tt]), 1e-37f);
+          const float score = fmaxf(fmaxf(x[n][tt][0], x[n][tt][1]), fmaxf(x[n][tt][2], x[n][tt][3]));
+          most = fmaxf(most, __builtin_fmaf(score, f[tt], (float)scale_exponent(vs[t0 + tt])));
+        }
         most = fmaxf(m[n], quarters_max(most));
         if (__builtin_amdgcn_ballot_w64(most > m[n])) {
           const float f = exp2_(m[n] - most);
@@ -349,8 +346,9 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
 #pragma unroll
         for (int tt = 0; tt < SUB; ++tt) {
           f4 p;
+          const float less = (float)scale_exponent(vs[t0 + tt]) - m[n];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] = exp2_(x[n][tt][i] - m[n]);
+          for (int i = 0; i < 4; ++i) p[i] = exp2_(__builtin_fmaf(x[n][tt][i], f[tt], less));
           l[n] = __builtin_fmaf((p[0] + p[1]) + (p[2] + p[3]), kx_bits_f32(scale_bits(-scale_exponent(vs[t0 + tt]))), l[n]);
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
@@ -584,7 +582,9 @@ int launch(KxPagedArgs a, int g, hipStream_t st) {
   const int units = (int)((std::max<long>(most, 1) + UNIT - 1) / UNIT);
   const long busy = (long)std::min(a.batch, a.tokens) * ((rows * g + FM::COLS - 1) / FM::COLS) * kv;  // workgroups of whole sequences
   const long room = std::min<long>({(long)(a.part_floats / FM::PART) / std::max<long>(1, tasks * kv), STATS / FM::COLS, units});
-  const long want = ((long)cus * FM::WAVES + busy - 1) / busy;
+  // a workgroup for each that the card holds; one a CU where a few long sequences fill it evenly: 1 x 131072 55.9 -> 52.5 us, 2 x 131072 88.4 -> 84.8, but 16 x 8192
+  // 41.7 -> 42.9 and 40 x 8192 95 -> 126, whose sequences differ in length
+  const long slots = (long)cus * (FM::ONCE && busy * 8 <= cus ? 1 : FM::WAVES), want = (slots + busy - 1) / busy;
   // a part has a group for each wave at least, and where more than 256 columns of parts are for one workgroup to add up, eight
   const long waves = FM::SHARE ? FM::NW : 1, most_parts = std::max(std::min<long>(units / waves, 256 / FM::COLS), units / (waves * 8));
   a.splits = (int)std::max<long>(1, std::min({room, want, most_parts}));
