@@ -442,6 +442,9 @@ extern "C" int kx_paged_faults(kx_paged *p, int32_t *h_bits, void *stream) {
   KX_REQUIRE(p && h_bits, "kx_paged_faults: null argument");
   KX_HIP(hipStreamSynchronize(kx_stream(stream)));
   KX_HIP(hipMemcpy(h_bits, p->a.fault, 4, hipMemcpyDeviceToHost));
-  if (*h_bits) KX_HIP(hipMemset(p->a.fault, 0, 4));
+  if (*h_bits) {
+    KX_HIP(hipMemset(p->a.fault, 0, 4));
+    KX_HIP(hipStreamSynchronize(nullptr));  // the next call may come on any stream
+  }
   return KX_OK;
 }
