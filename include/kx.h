@@ -389,7 +389,8 @@ int kx_linear_run(const kx_linear_args *args, void *d_row_scratch, void *stream)
  *   (t / 4 % 4) 16 + t / 32 8 + t / 16 % 2 4 + t % 4 of a row of d_v.
  *   d_k_scale, d_v_scale f32 [pages][kv_heads][page / block]: an element is its code times the scale of its block of 16, 32 or 64 positions,
  *   2^e with the least e >= -100 that keeps the block's largest finite magnitude within 448 * 2^e.
- * Nothing has to be initialised, and d_k and d_v begin at multiples of 16 bytes.  The rows of a call are those of a ragged batch: sequence b has rows d_start[b] .. d_start[b + 1] - 1 (d_start i32 [batch + 1]), at
+ * Nothing has to be initialised, and d_k and d_v begin at multiples of 16 bytes.
+ * The rows of a call are those of a ragged batch: sequence b has rows d_start[b] .. d_start[b + 1] - 1 (d_start i32 [batch + 1]), at
  * positions from d_pos[b] on (i32 [batch]); a sequence may have none.  `tokens`: rows that there is memory for; rows behind d_start[batch]
  * are not read or written.  `longest`: positions of the longest sequence, the new ones among them, by which the work is shared out; a longer one costs time
  * and nothing else.  Tables lie on the device, so that a captured call replays with other lengths and pages.
