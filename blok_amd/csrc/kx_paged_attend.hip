@@ -2,8 +2,8 @@
 // in the reference, whose attention goes over 32-bit tiles of one sequence (tiled_attention, src/kimi_exec.cu:692-716).
 //
 // With codes k, v and scales 2^a, 2^b of a token's blocks, and all in powers of two: x_t = (q . k_t) 2^a scale log2(e) + b,
-//   out = sum_t 2^(x_t - M) v_t / sum_t 2^(x_t - b - M),  M the largest x so far.
-// The values' scale is a part of the exponent, so that the products with the values are of codes as they are and the largest weight is 1.
+//   out = sum_t 2^(x_t - M) v_t / sum_t 2^(x_t - b - M),  M at most 8 below the largest x so far.
+// The values' scale is a part of the exponent, so that the products with the values are of codes as they are and the largest weight lies between 1 and 2^8.
 // A wave has 16 NQ columns -- a column is a query head of a row, all of them of one head of keys -- and goes through groups of 64 tokens on its own:
 //   S^T = K Q^T (v_mfma_f32_16x16x32_f16) leaves each lane scores of one column and of 4 tokens of each block of 16, which is the operand that
 //   O^T += V^T P^T wants, with the values' tokens in the order of kxpage::place_of.  Nothing passes through LDS or between lanes but the largest x.
@@ -36,6 +36,7 @@ struct Scales {
 };
 
 constexpr float NONE = -1e30f;  // M where nothing has been seen
+constexpr float GROWTH = 8.0f;  // by so much x may be above M before the sums are divided by what M grows: weights are 2^8 at most
 constexpr int STATS = 4096;     // columns times parts of a task
 
 __device__ __forceinline__ h8 unpacked(uint32_t lo, uint32_t hi) {
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
           most = fmaxf(most, __builtin_fmaf(score, f[tt], (float)scale_exponent(vs[t0 + tt])));
         }
         most = fmaxf(m[n], quarters_max(most));
-        if (__builtin_amdgcn_ballot_w64(most > m[n])) {
+        if (__builtin_amdgcn_ballot_w64(most > m[n] + GROWTH)) {
           const float f = exp2_(m[n] - most);
           m[n] = most;
           l[n] *= f;
