@@ -32,7 +32,7 @@ struct KxPagedArgs {
   void *out = nullptr;           // attention: [tokens][out_ld] of the number format; read: keys
   void *out_v = nullptr;         // read: values
   int out_ld = 0, out_v_ld = 0;
-  bool wide_k = false, wide_v = false;  // read: rows of results are whole pieces of 16 bytes
+  bool wide_k = false, wide_v = false;  // rows of results are whole pieces: of 16 bytes read, of 4 elements of an attention
   int *fault = nullptr;          // KX_PAGED_* bits
   // attention: sums of parts of the positions, and who has handed his in
   float *part = nullptr;

@@ -412,6 +412,12 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
   auto give = [&](int c, int d, f4 y) {  // column c of the sequence, dimensions d .. d + 3
     const int at = row_of(c);
     const size_t to = (size_t)(t.r.first + at) * a.out_ld + (size_t)(head * g + c - at * g) * s.vdim + d;
+    if (a.wide_v) {
+      if (d >= s.vdim) return;
+      if constexpr (F32) *(f4 *)((float *)a.out + to) = y;
+      else *(uint2 *)((uint16_t *)a.out + to) = make_uint2(kx_bf16_rne(y[0]) | (uint32_t)kx_bf16_rne(y[1]) << 16, kx_bf16_rne(y[2]) | (uint32_t)kx_bf16_rne(y[3]) << 16);
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (d + e < s.vdim) {

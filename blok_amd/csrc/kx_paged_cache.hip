@@ -436,6 +436,7 @@ extern "C" int kx_paged_attend(kx_paged *p, const kx_paged_cache *cache, const k
   if (!a.tokens) return KX_OK;
   a.proj = (const float *)d_proj; a.proj_ld = proj_ld; a.q_off = q_off;
   a.out = d_out; a.out_ld = out_ld;
+  a.wide_v = (uintptr_t)d_out % (p->f32 ? 16 : 8) == 0 && out_ld % 4 == 0 && a.s.vdim % 4 == 0;
   return kx_paged_attend_launch(p->f32, a, kx_stream(stream));
 }
 extern "C" int kx_paged_faults(kx_paged *p, int32_t *h_bits, void *stream) {
