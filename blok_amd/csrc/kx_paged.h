@@ -48,6 +48,7 @@ int kx_paged_read_launch(const KxPagedArgs &a, hipStream_t st);
 int kx_paged_attend_launch(bool f32, const KxPagedArgs &a, hipStream_t st);
 // counters and floats of parts that steps of up to max_tokens rows of max_batch sequences can use
 int kx_paged_arrivals(const KxPagedSpec &s, int max_batch, int max_tokens);
+size_t kx_paged_part_floats(const KxPagedSpec &s, int max_batch, int max_tokens);
 
 namespace kxpage {
 inline KxDivider divider(int d) { return {d, 0xffffffffu / (uint32_t)d}; }

@@ -592,8 +592,10 @@ int launch(KxPagedArgs a, int g, hipStream_t st) {
   // a workgroup for each that the card holds; one a CU where a few long sequences fill it evenly: 1 x 131072 55.9 -> 52.5 us, 2 x 131072 88.4 -> 84.8, but 16 x 8192
   // 41.7 -> 42.9 and 40 x 8192 95 -> 126, whose sequences differ in length
   const long slots = (long)cus * (FM::ONCE && busy * 8 <= cus ? 1 : FM::WAVES), want = (slots + busy - 1) / busy;
-  // a part has a group for each wave at least, and where more than 256 columns of parts are for one workgroup to add up, eight
-  const long waves = FM::SHARE ? FM::NW : 1, most_parts = std::max(std::min<long>(units / waves, 256 / FM::COLS), units / (waves * 8));
+  // Where waves share columns, a part has a group for each at least, and where more than 256 columns of parts are for one workgroup to add up, eight.  Where
+  // they do not, adding up 128 columns takes as long as 12 groups, and a part has 20: 256 rows after 7744, 6 parts 245 -> 126 us, 100 rows after 7900 231 -> 86,
+  // but 300 rows after 1700 in 2 parts 69 -> 77, 100 rows after 500 31 -> 37.
+  const long most_parts = FM::SHARE ? std::max<long>(std::min<long>(units / FM::NW, 256 / FM::COLS), units / (FM::NW * 8)) : units / 20;
   a.splits = (int)std::max<long>(1, std::min({room, want, most_parts}));
   a.chunk = (units + a.splits - 1) / a.splits;
   a.by_splits = divider(a.splits);
@@ -628,5 +630,11 @@ int launch_widths(const KxPagedArgs &a, hipStream_t st) {
 int kx_paged_arrivals(const KxPagedSpec &s, int max_batch, int max_tokens) {
   const long tasks = (long)std::min(max_batch, max_tokens) + (long)max_tokens * (s.heads / s.kv_heads) / 16;
   return (int)std::min<long>(tasks * s.kv_heads, 0x7fffffff);
+}
+// room for the parts of 512 workgroups of 64 columns of 128 dimensions, or for all sums of four times a call whose sequences have more than 64 columns, 128 MB at most
+size_t kx_paged_part_floats(const KxPagedSpec &s, int max_batch, int max_tokens) {
+  const size_t g = (size_t)(s.heads / s.kv_heads), least = (size_t)512 * 64 * 130, most = (size_t)1 << 25;
+  const size_t sequences = std::min<size_t>((size_t)std::min(max_batch, max_tokens), (size_t)max_tokens * g / 64 + 1);
+  return std::max(least, std::min(most, 4 * (size_t)(s.vp + 2) * ((size_t)max_tokens * (size_t)s.heads + 128 * (size_t)s.kv_heads * sequences)));
 }
 int kx_paged_attend_launch(bool f32, const KxPagedArgs &a, hipStream_t st) { return f32 ? launch_widths<true>(a, st) : launch_widths<false>(a, st); }

@@ -326,9 +326,6 @@ struct kx_paged {
 
 namespace {
 
-// floats for the sums of parts: 256 CUs times two workgroups with 64 columns of 128 dimensions each
-constexpr size_t PART_FLOATS = (size_t)512 * 64 * 130;
-
 int common(const char *who, kx_paged *p, const kx_paged_cache *c, const kx_paged_rows *r, KxPagedArgs *out) {
   KX_REQUIRE(p && c && r, "%s: null argument", who);
   KX_REQUIRE(c->d_k && c->d_v && c->d_k_scale && c->d_v_scale && c->d_table && r->d_start && r->d_pos, "%s: null pointer in the cache or the rows", who);
@@ -378,11 +375,11 @@ extern "C" int kx_paged_create(const kx_paged_config *c, const double *h_freq, i
     p->f32 = f32 != 0;
     p->max_batch = max_batch; p->max_tokens = max_tokens;
     p->a.arrivals = kx_paged_arrivals(s, max_batch, max_tokens);
-    p->a.part_floats = PART_FLOATS;
+    p->a.part_floats = kx_paged_part_floats(s, max_batch, max_tokens);
     const size_t turns = (turn.size() * 8 + 255) & ~(size_t)255, counters = ((size_t)p->a.arrivals * 4 + 4 + 255) & ~(size_t)255;
     KX_HIP(hipGetDevice(&p->device));
-    if (hipMalloc((void **)&p->mem, turns + counters + PART_FLOATS * 4) != hipSuccess) {
-      kx_set_error("kx_paged_create: no device memory for %zu bytes", turns + counters + PART_FLOATS * 4);
+    if (hipMalloc((void **)&p->mem, turns + counters + p->a.part_floats * 4) != hipSuccess) {
+      kx_set_error("kx_paged_create: no device memory for %zu bytes", turns + counters + p->a.part_floats * 4);
       return KX_ERR_HIP;
     }
     p->a.turn = (const double *)p->mem;

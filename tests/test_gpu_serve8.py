@@ -242,3 +242,21 @@ def test_rows_read_into_aligned_pieces(kxlib):
         np.testing.assert_array_equal(S.bf16(k[:, :128]).reshape(79, 2, 64), np.concatenate([h[0] for h in held]))
         np.testing.assert_array_equal(S.bf16(v[:, :80]).reshape(79, 2, 40), np.concatenate([h[1] for h in held]))
     p.close()
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("shape", [dict(dim=64, vdim=64, rot=64), dict(dim=128, vdim=100, rot=64, block=64), dict(dim=192, vdim=128, size=700), dict(dim=200, vdim=256, block=16)], ids=lambda s: str(s["dim"]))
+def test_many_rows_behind_many_positions(kxlib, f32, shape):
+    """Columns that waves have for themselves, their positions split between workgroups; the same bits again."""
+    say(f"many rows {shape} f32={f32}")
+    p = S.Paged(kxlib, heads=4, kv=1, batch=2, f32=f32, tokens=2700, pages=60, seed=8, **shape)
+    lens, new = [2600, 100], [39, 35]
+    p.append(lens, [0, 0])
+    pos, q = [n - m for n, m in zip(lens, new)], p.queries(sum(new))
+    got = p.attend(new, pos, q)
+    y, tol = p.expect(new, pos, q)
+    Layer.close_to("attention", got, y, tol)
+    for _ in range(3):
+        np.testing.assert_array_equal(p.attend(new, pos, q), got)
+    assert p.faults() == 0
+    p.close()
