@@ -11,6 +11,9 @@
 // the bf16 result; in the 32-bit format both are the sum of two f16, 2^-22).  Sums, M and denominators are 32-bit.
 // Two forms: few columns a sequence (SHARE): the waves of a workgroup take groups of tokens in turn and are added up in LDS; many: every wave has columns
 // of its own.  In both the positions may be split between workgroups, and the last one in adds the parts (kx_arrive.h), in order.
+// What bounds it: few columns, HBM -- one position after 131072, 269 MB, 52 us, 11 of them the start and the parts; 64 sequences of up to 8192, 640 MB, 124 us, whose
+// lengths differ -- and for short caches the chain from the tables to the pages and the hand-over, 11 us after 4096.  Many columns, vector instructions beside the
+// matrix cores (128 conversions of codes and 32 exponentials for 64 products of a wave): 590 TFLOP/s of 1200.
 #include <algorithm>
 #include <type_traits>
 #include "kx_arrive.h"
