@@ -615,7 +615,8 @@ int launch_columns(const KxPagedArgs &a, hipStream_t st) {
   constexpr int NQ = DP == 256 ? 1 : 2;  // the widest rows leave registers for one block of columns
   // a cache that no level of caches holds is read past them where one workgroup reads each of its positions: 269 MB 62 -> 56 us, 640 MB 128 -> 124; with 131 MB,
   // which the last level holds from one call to the next in a program of one layer, it takes 27 us instead of 24
-  if (columns <= 16 && kxonce::latent((size_t)std::min(a.batch, a.tokens) * a.longest * a.s.kv_heads * (DP + VP))) return launch<Form<DP, VP, 1, true, F32, true>>(a, g, st);
+  const size_t seen = a.s.size ? std::min(a.longest, a.s.size) : a.longest;
+  if (columns <= 16 && kxonce::latent((size_t)std::min(a.batch, a.tokens) * seen * a.s.kv_heads * (DP + VP))) return launch<Form<DP, VP, 1, true, F32, true>>(a, g, st);
   if (columns <= 16) return launch<Form<DP, VP, 1, true, F32>>(a, g, st);
   if (columns <= 64) return launch<Form<DP, VP, NQ, true, F32>>(a, g, st);
   return launch<Form<DP, VP, NQ, false, F32>>(a, g, st);
@@ -634,7 +635,8 @@ int kx_paged_arrivals(const KxPagedSpec &s, int max_batch, int max_tokens) {
   const long tasks = (long)std::min(max_batch, max_tokens) + (long)max_tokens * (s.heads / s.kv_heads) / 16;
   return (int)std::min<long>(tasks * s.kv_heads, 0x7fffffff);
 }
-// room for the parts of 512 workgroups of 64 columns of 128 dimensions, or for all sums of four times a call whose sequences have more than 64 columns, 128 MB at most
+// room for a part of each of 512 workgroups of 64 columns of 128 dimensions, or for four parts of every column, those of partly filled blocks among them, in calls
+// whose sequences have more than 64; 128 MB at most
 size_t kx_paged_part_floats(const KxPagedSpec &s, int max_batch, int max_tokens) {
   const size_t g = (size_t)(s.heads / s.kv_heads), least = (size_t)512 * 64 * 130, most = (size_t)1 << 25;
   const size_t sequences = std::min<size_t>((size_t)std::min(max_batch, max_tokens), (size_t)max_tokens * g / 64 + 1);
