@@ -2,13 +2,16 @@
 // in the reference, whose attention goes over 32-bit tiles of one sequence (tiled_attention, src/kimi_exec.cu:692-716).
 //
 // With codes k, v and scales 2^a, 2^b of a token's blocks, and all in powers of two: x_t = (q . k_t) 2^a scale log2(e) + b,
-//   out = sum_t 2^(x_t - M) v_t / sum_t 2^(x_t - b - M),  M at most 8 below the largest x so far.
-// The values' scale is a part of the exponent, so that the products with the values are of codes as they are and the largest weight lies between 1 and 2^8.
+//   out = sum_t 2^(x_t - M) v_t / sum_t 2^(x_t - b - M),  M at most 4 below the largest x so far.
+// The values' scale is a part of the exponent, so that the products with the values are of codes and the largest of these weights lies between 1 and 2^4.
 // A wave has 16 NQ columns -- a column is a query head of a row, all of them of one head of keys -- and goes through groups of 64 tokens on its own:
 //   S^T = K Q^T (v_mfma_f32_16x16x32_f16) leaves each lane scores of one column and of 4 tokens of each block of 16, which is the operand that
 //   O^T += V^T P^T wants, with the values' tokens in the order of kxpage::place_of.  Nothing passes through LDS or between lanes but the largest x.
-// Codes become f16 in registers, exactly; a query is divided by a power of two and rounded to f16, weights likewise (2^-12 of each, against the 2^-9 of
-// the bf16 result; in the 32-bit format both are the sum of two f16, 2^-22).  Sums, M and denominators are 32-bit.
+// Codes become f16 in registers, exactly; a query is divided by a power of two and rounded to f16 (2^-11 of an element, against the 2^-8 of the bf16 result; in the
+// 32-bit format it is the sum of two, 2^-22).  For bf16 results weights times 2^11, which is taken out of the values' codes, are rounded to f16, too: 2^-11 of each
+// that is at least 2^-25 of the largest, and 2^-36 of the largest below that.  Many small weights beside a large one make a result as well: in the 32-bit format, a
+// weight is the sum of three bf16, which hold any float, and costs two more products (4 sequences of 300 rows after 2700, 177 us with two f16, 203 with three bf16).
+// Sums, M and denominators are 32-bit.
 // Two forms: few columns a sequence (SHARE): the waves of a workgroup take groups of tokens in turn and are added up in LDS; many: every wave has columns
 // of its own.  In both the positions may be split between workgroups, and the last one in adds the parts (kx_arrive.h), in order.
 // What bounds it: few columns, HBM -- one position after 131072, 269 MB, 52 us, 11 of them the start and the parts; 64 sequences of up to 8192, 640 MB, 124 us, whose
@@ -29,6 +32,8 @@ using namespace kxpage;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
@@ -39,7 +44,8 @@ struct Scales {
 };
 
 constexpr float NONE = -1e30f;  // M where nothing has been seen
-constexpr float GROWTH = 8.0f;  // by so much x may be above M before the sums are divided by what M grows: weights are 2^8 at most
+constexpr float GROWTH = 4.0f;  // by so much x may be above M before the sums are divided by what M grows
+constexpr int ROOM = 11;        // weights are times 2^ROOM beside the matrix cores: the largest at least that, and below 2^15.  7 beside a growth of 8, and 13 beside 2, are as fast
 constexpr int STATS = 4096;     // columns times parts of a task
 
 __device__ __forceinline__ h8 unpacked(uint32_t lo, uint32_t hi) {
@@ -47,7 +53,21 @@ __device__ __forceinline__ h8 unpacked(uint32_t lo, uint32_t hi) {
   const h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, true);
   return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+// codes divided by 2^ROOM, exactly: the smallest is 2^-9, and f16 has 2^-24
+__device__ __forceinline__ h8 unpacked_down(uint32_t lo, uint32_t hi) {
+  constexpr float down = 1.0f / (1 << ROOM);
+  const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, down, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, down, true);
+  const h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, down, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, down, true);
+  return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ b8 unpacked_down_wide(uint32_t lo, uint32_t hi) {  // as bf16
+  constexpr float down = 1.0f / (1 << ROOM);
+  const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, down, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, down, true);
+  const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, down, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, down, true);
+  return b8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
 __device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4 mfma(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 // over the four quarters of the wave
 __device__ __forceinline__ float quarters_max(float v) {
   float o = v;
@@ -320,7 +340,8 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
         load_k(u + STEP, next);
         sc = load_scales(u + STEP, next);
       }
-      h8 ph[NQ][SUB / 2], pl[F32 ? NQ : 1][SUB / 2];
+      typedef std::conditional_t<F32, b8, h8> P8;
+      P8 ph[NQ][SUB / 2], pm[F32 ? NQ : 1][SUB / 2], pl[F32 ? NQ : 1][SUB / 2];
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
         if (!whole) {
@@ -350,19 +371,28 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
 #pragma unroll
         for (int tt = 0; tt < SUB; ++tt) {
           f4 p;
-          const float less = (float)scale_exponent(vs[t0 + tt]) - m[n];
+          const float less = (float)(scale_exponent(vs[t0 + tt]) + ROOM) - m[n];
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[i] = exp2_(__builtin_fmaf(x[n][tt][i], f[tt], less));
-          l[n] = __builtin_fmaf((p[0] + p[1]) + (p[2] + p[3]), kx_bits_f32(scale_bits(-scale_exponent(vs[t0 + tt]))), l[n]);
+          l[n] += __builtin_amdgcn_ldexpf((p[0] + p[1]) + (p[2] + p[3]), -(scale_exponent(vs[t0 + tt]) + ROOM));
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
-            const h2 h = halves_of(p[i], p[i + 1]);
-            ph[n][tt >> 1][(tt & 1) * 4 + i] = h[0];
-            ph[n][tt >> 1][(tt & 1) * 4 + i + 1] = h[1];
-            if constexpr (F32) {
-              const h2 r = halves_of(p[i] - (float)h[0], p[i + 1] - (float)h[1]);
-              pl[n][tt >> 1][(tt & 1) * 4 + i] = r[0];
-              pl[n][tt >> 1][(tt & 1) * 4 + i + 1] = r[1];
+            auto put = [&](P8 &to, auto w) {
+              to[(tt & 1) * 4 + i] = w[0];
+              to[(tt & 1) * 4 + i + 1] = w[1];
+            };
+            if constexpr (F32) {  // three bf16 hold a float
+              float a = p[i], b = p[i + 1];
+              auto next = [&](P8 &to) {
+                const b2 w = __builtin_convertvector((f2{a, b}), b2);
+                put(to, w);
+                a -= (float)w[0], b -= (float)w[1];
+              };
+              next(ph[n][tt >> 1]);
+              next(pm[n][tt >> 1]);
+              next(pl[n][tt >> 1]);
+            } else {
+              put(ph[n][tt >> 1], halves_of(p[i], p[i + 1]));
             }
           }
         }
@@ -371,11 +401,14 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
       for (int i = 0; i < VP / 16; ++i)
 #pragma unroll
         for (int h = 0; h < SUB / 2; ++h) {
-          const h8 v = t0 / 2 + h == 0 ? unpacked(vr[i].x, vr[i].y) : unpacked(vr[i].z, vr[i].w);
+          const uint32_t lo = t0 / 2 + h == 0 ? vr[i].x : vr[i].z, hi = t0 / 2 + h == 0 ? vr[i].y : vr[i].w;
+          P8 v;
+          if constexpr (F32) v = unpacked_down_wide(lo, hi);
+          else v = unpacked_down(lo, hi);
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {
             o[n][i] = mfma(v, ph[n][h], o[n][i]);
-            if constexpr (F32) o[n][i] = mfma(v, pl[n][h], o[n][i]);
+            if constexpr (F32) o[n][i] = mfma(v, pl[n][h], mfma(v, pm[n][h], o[n][i]));
           }
         }
     }

@@ -396,8 +396,10 @@ int kx_linear_run(const kx_linear_args *args, void *d_row_scratch, void *stream)
  * and nothing else.  Tables lie on the device, so that a captured call replays with other lengths and pages.
  * kx_paged_create: handle with scratch for calls of up to max_batch sequences and, appending and attending, max_tokens rows, on the current device.  Queries and keys
  *   are turned by their positions: the first `rot` dimensions in pairs (d, d + rot / 2), with pairs = 1 (2 d, 2 d + 1), by position * h_freq[d]
- *   (rot / 2 doubles), or base^(-2 d / rot) where h_freq is NULL.  f32: results are float, and as exact; 0: bf16.  Calls on
- *   one handle that overlap (two streams, two threads, two graphs) race; calls one after another do not.  One handle serves any number of caches.
+ *   (rot / 2 doubles), or base^(-2 d / rot) where h_freq is NULL.  f32: results are float, of queries in 22 bits and weights in 32; 0: bf16, of
+ *   queries and weights in f16, where a weight w of a position whose values have the scale 2^e is off by 2^-11 of itself or 2^-36 of the largest w 2^e divided by
+ *   its own 2^e.  Calls on one handle that overlap (two streams, two threads, two graphs) race; calls one after another do not.  One handle serves any
+ *   number of caches.
  * kx_paged_append: d_proj f32 [tokens][proj_ld] holds the rows' keys [kv_heads][dim] from column k_off on and values [kv_heads][vdim] from
  *   v_off on.  A block that the new rows begin takes its scale from them; one that has older tokens keeps its scale or, if they need a
  *   larger one, has its older codes divided by what it grew.  Positions behind the last appended one hold nothing from then on.  What is not finite
