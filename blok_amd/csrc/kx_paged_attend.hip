@@ -46,6 +46,8 @@ struct Scales {
 constexpr float NONE = -1e30f;  // M where nothing has been seen
 constexpr float GROWTH = 4.0f;  // by so much x may be above M before the sums are divided by what M grows
 constexpr int ROOM = 11;        // weights are times 2^ROOM beside the matrix cores: the largest at least that, and below 2^15.  7 beside a growth of 8, and 13 beside 2, are as fast
+constexpr int FAR = 96;         // where a block's scale is so many powers of two below the largest so far (values of zero have the least), a weight times its scale may be no float
+                                // any more and the weight still count: such weights go into the denominator without it.  The test costs 1 % where columns are many
 constexpr int STATS = 4096;     // columns times parts of a task
 
 __device__ __forceinline__ h8 unpacked(uint32_t lo, uint32_t hi) {
@@ -85,6 +87,13 @@ __device__ __forceinline__ float quarters_sum(float v) {
 }
 __device__ __forceinline__ h2 halves_of(float a, float b) { return __builtin_convertvector((f2{a, b}), h2); }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// x without what a weight has of the values' scale 2^e and of ROOM
+__device__ __forceinline__ float unscaled(float x, uint32_t scale) { return __builtin_amdgcn_ldexpf(x, -(scale_exponent(scale) + ROOM)); }
+// x 2^d for a d that may lie below the exponents of floats
+__device__ __forceinline__ float lowered(float x, float d) {
+  const float f = exp2_(0.5f * d);
+  return x * f * f;
+}
 
 template <bool ONCE>
 __device__ __forceinline__ uint4 piece(const uint8_t *p) {
@@ -281,6 +290,7 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
 
   // a group, SUB blocks of 16 at a time
   constexpr int SUB = FM::SUB;
+  int most_scale = kxpage::LEAST;  // largest exponent of the values' scales so far
   for (int u = u_from; u < u_to; u += STEP) {
     const bool there = page_ok(id, a.pages);
     const int base = u * UNIT, after = page_at(u + 2 * STEP);
@@ -340,6 +350,14 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
         load_k(u + STEP, next);
         sc = load_scales(u + STEP, next);
       }
+      int least_scale = scale_exponent(vs[t0]);
+      most_scale = max(most_scale, least_scale);
+#pragma unroll
+      for (int tt = 1; tt < SUB; ++tt) {
+        most_scale = max(most_scale, scale_exponent(vs[t0 + tt]));
+        least_scale = min(least_scale, scale_exponent(vs[t0 + tt]));
+      }
+      const bool far = most_scale - least_scale > FAR;
       typedef std::conditional_t<F32, b8, h8> P8;
       P8 ph[NQ][SUB / 2], pm[F32 ? NQ : 1][SUB / 2], pl[F32 ? NQ : 1][SUB / 2];
 #pragma unroll
@@ -361,12 +379,20 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
           most = fmaxf(most, __builtin_fmaf(score, f[tt], (float)scale_exponent(vs[t0 + tt])));
         }
         most = fmaxf(m[n], quarters_max(most));
-        if (__builtin_amdgcn_ballot_w64(most > m[n] + GROWTH)) {
-          const float f = exp2_(m[n] - most);
+        if (far || __builtin_amdgcn_ballot_w64(most > m[n] + GROWTH)) {
+          const float less = m[n] - most, shrink = exp2_(less);
           m[n] = most;
-          l[n] *= f;
+          l[n] = lowered(l[n], less);
 #pragma unroll
-          for (int v = 0; v < VP / 16; ++v) o[n][v] *= f;
+          for (int v = 0; v < VP / 16; ++v) o[n][v] *= shrink;
+          if (far) {
+#pragma unroll
+            for (int tt = 0; tt < SUB; ++tt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)  // the weight, and what will be added below instead of it
+                l[n] += exp2_(__builtin_fmaf(x[n][tt][i], f[tt], -m[n])) -
+                        unscaled(exp2_(__builtin_fmaf(x[n][tt][i], f[tt], (float)(scale_exponent(vs[t0 + tt]) + ROOM) - m[n])), vs[t0 + tt]);
+          }
         }
 #pragma unroll
         for (int tt = 0; tt < SUB; ++tt) {
@@ -374,7 +400,7 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
           const float less = (float)(scale_exponent(vs[t0 + tt]) + ROOM) - m[n];
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[i] = exp2_(__builtin_fmaf(x[n][tt][i], f[tt], less));
-          l[n] += __builtin_amdgcn_ldexpf((p[0] + p[1]) + (p[2] + p[3]), -(scale_exponent(vs[t0 + tt]) + ROOM));
+          l[n] += unscaled((p[0] + p[1]) + (p[2] + p[3]), vs[t0 + tt]);
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
             auto put = [&](P8 &to, auto w) {
@@ -495,7 +521,7 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
 #pragma unroll
           for (int w = 0; w < NW; ++w) {
             const float f = exp2_(st[w].x - most);
-            sum = __builtin_fmaf(st[w].y, f, sum);
+            sum += lowered(st[w].y, st[w].x - most);
             const f4 x = *(const f4 *)(lds + (w * 16 + c) * FM::OLD + d);
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(x[e], f, y[e]);
@@ -555,7 +581,7 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
       for (int p = lc; p < used; p += 16) most = fmaxf(most, st[p * COLS + c].x);
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-      for (int p = lc; p < used; p += 16) sum = __builtin_fmaf(st[p * COLS + c].y, exp2_(st[p * COLS + c].x - most), sum);
+      for (int p = lc; p < used; p += 16) sum += lowered(st[p * COLS + c].y, st[p * COLS + c].x - most);
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d);
       const float f = sum == 0.0f ? 0.0f : 1.0f / sum;

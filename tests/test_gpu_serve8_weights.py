@@ -96,3 +96,25 @@ def test_many_positions_far_below_one(kxlib, rows, heads, bits, f32):
         near(attend(p, [rows], [n - rows], q, longest), expect(p, [rows], [n - rows], q), f"longest {longest}")
     assert p.faults() == 0
     p.close()
+
+
+@FORMATS
+@pytest.mark.parametrize("rows,heads", ROWS)
+@pytest.mark.parametrize("large", [1.0, 1e14, 1e30])
+@pytest.mark.parametrize("first", [False, True])
+def test_values_of_zero_beside_large_ones(kxlib, rows, heads, large, first, f32):
+    """Positions whose values are zero, in blocks whose scale is the least there is, have their share of the weights whatever the others' values are."""
+    say(f"{rows} rows of {heads} heads, values of {large}, zeros first={first}, f32={f32}")
+    n = 700
+    p = S.Paged(kxlib, heads=heads, kv=1, dim=64, vdim=64, block=64, f32=f32, tokens=n, pages=12)
+    r = np.random.default_rng(3)
+    k, v = r.standard_normal((n, 1, 64)).astype(np.float32), (large * (1 + 0.3 * r.standard_normal((n, 1, 64)))).astype(np.float32)
+    v[:320] = 0.0
+    if not first:
+        v = v[::-1].copy()
+        v[n - 320 // 64 * 64 + 60:] = 0.0
+    p.append([n], [0], k=k, v=v)
+    q = p.queries(rows, 0.3)
+    for longest in (1, n):
+        near(attend(p, [rows], [n - rows], q, longest), expect(p, [rows], [n - rows], q), f"longest {longest}")
+    p.close()
