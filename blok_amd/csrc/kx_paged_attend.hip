@@ -7,8 +7,8 @@
 // A wave has 16 NQ columns -- a column is a query head of a row, all of them of one head of keys -- and goes through groups of 64 tokens on its own:
 //   S^T = K Q^T (v_mfma_f32_16x16x32_f16) leaves each lane scores of one column and of 4 tokens of each block of 16, which is the operand that
 //   O^T += V^T P^T wants, with the values' tokens in the order of kxpage::place_of.  Nothing passes through LDS or between lanes but the largest x.
-// Codes become f16 in registers, exactly; a query is divided by a power of two and rounded to f16 (2^-11 of an element, against the 2^-8 of the bf16 result; in the
-// 32-bit format it is the sum of two, 2^-22).  For bf16 results weights times 2^11, which is taken out of the values' codes, are rounded to f16, too: 2^-11 of each
+// Codes become f16 in registers, exactly; a query is divided by a power of two and rounded to f16 (2^-11 of an element or 2^-39 of its largest, against the 2^-8 of the bf16
+// result; in the 32-bit format it is the sum of two, 2^-22 of an element).  For bf16 results weights times 2^11, which is taken out of the values' codes, are rounded to f16, too: 2^-11 of each
 // that is at least 2^-25 of the largest, and 2^-36 of the largest below that.  Many small weights beside a large one make a result as well: in the 32-bit format, a
 // weight is the sum of three bf16, which hold any float, and costs two more products (4 sequences of 300 rows after 2700, 177 us with two f16, 203 with three bf16).
 // Sums, M and denominators are 32-bit.
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
           most = fmaxf(most, x < __builtin_inff() ? x : 0.0f);
         }
       most = quarters_max(most);
-      const int e = max(min((int)(kx_f32_bits(most) >> 23) - 126, 120), -100);
+      const int e = max((int)(kx_f32_bits(most) >> 23) - 141, -100);  // the largest element becomes 2^14 or more: f16 has 2^-24 beside it
       const float down = s.scale == 0.0f ? 0.0f : __builtin_copysignf(kx_bits_f32(scale_bits(-e)), s.scale);
       qf[n] = kx_bits_f32(scale_bits(e)) * __builtin_fabsf(s.scale) * 1.44269504088896341f;
 #pragma unroll

@@ -100,6 +100,23 @@ def test_many_positions_far_below_one(kxlib, rows, heads, bits, f32):
 
 @FORMATS
 @pytest.mark.parametrize("rows,heads", ROWS)
+@pytest.mark.parametrize("bits", [20, 24])
+def test_queries_with_one_large_element(kxlib, rows, heads, bits, f32):
+    """An element of a query that meets keys of zero and is 2^bits times as large as the others takes nothing from these."""
+    say(f"{rows} rows of {heads} heads, an element of 2^{bits}, f32={f32}")
+    n = 400
+    p = S.Paged(kxlib, heads=heads, kv=1, dim=64, vdim=64, block=32, f32=f32, tokens=n, pages=8)
+    k = np.random.default_rng(bits).standard_normal((n, 1, 64)).astype(np.float32)
+    k[:, 0, 5] = 0.0
+    p.append([n], [0], k=k, v=k[::-1].copy())
+    q = p.queries(rows, 1.0)
+    q[:, 2 + 5:2 + heads * 64:64] = 2.0 ** bits
+    near(attend(p, [rows], [n - rows], q), expect(p, [rows], [n - rows], q))
+    p.close()
+
+
+@FORMATS
+@pytest.mark.parametrize("rows,heads", ROWS)
 @pytest.mark.parametrize("large", [1.0, 1e14, 1e30])
 @pytest.mark.parametrize("first", [False, True])
 def test_values_of_zero_beside_large_ones(kxlib, rows, heads, large, first, f32):
