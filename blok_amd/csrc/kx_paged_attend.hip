@@ -253,17 +253,20 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
 #pragma unroll
     for (int n = n0; n < (SHARE ? NQ : n0 + 1); ++n) {
       float most = 0.0f;
+      bool finite = true;
       const float *const mine = rows + ((n - n0) * 16 + lc) * FM::QLD + lq * 16;
 #pragma unroll
       for (int j = 0; j < DP / 64; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float x = __builtin_fabsf(mine[j * 64 + e]);
+          finite &= x < __builtin_inff();
           most = fmaxf(most, x < __builtin_inff() ? x : 0.0f);
         }
       most = quarters_max(most);
       const int e = max((int)(kx_f32_bits(most) >> 23) - 141, -100);  // the largest element becomes 2^14 or more: f16 has 2^-24 beside it
-      const float down = s.scale == 0.0f ? 0.0f : __builtin_copysignf(kx_bits_f32(scale_bits(-e)), s.scale);
+      // a query that is not finite has infinite scores or none, and NaN for their softmax: NaN in any element, where minus infinity would hide its positions
+      const float down = !finite ? __builtin_nanf("") : s.scale == 0.0f ? 0.0f : __builtin_copysignf(kx_bits_f32(scale_bits(-e)), s.scale);
       qf[n] = kx_bits_f32(scale_bits(e)) * __builtin_fabsf(s.scale) * 1.44269504088896341f;
 #pragma unroll
       for (int j = 0; j < DP / 64; ++j)

@@ -406,7 +406,7 @@ int kx_linear_run(const kx_linear_args *args, void *d_row_scratch, void *stream)
  *   is NaN in the cache.  Two sequences of a call must not append to the same page.
  * kx_paged_attend: out = softmax(scale q k^T) v over the positions up to a row's own, the last `size` of them where size > 0; queries [heads][dim] of
  *   d_proj from q_off on, d_out [tokens][out_ld] of heads * vdim.  Head h reads head h / (heads / kv_heads) of keys.  The rows' own keys and
- *   values have been appended before.
+ *   values have been appended before.  The results of a query with an element that is not finite are NaN.
  * kx_paged_read: the keys and values that the cache has at the rows' positions, bf16 [tokens][k_ld] and [tokens][v_ld].
  * kx_paged_faults: whether the tables of earlier calls held a page outside [0, pages) (KX_PAGED_BAD_PAGE: appended rows are dropped, its positions are not
  *   seen), positions outside the table (_BAD_POSITION) or rows outside [0, tokens] (_BAD_ROWS; such sequences are left out).  Synchronises, and clears them.  A result that

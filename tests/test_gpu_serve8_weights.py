@@ -135,3 +135,27 @@ def test_values_of_zero_beside_large_ones(kxlib, rows, heads, large, first, f32)
     for longest in (1, n):
         near(attend(p, [rows], [n - rows], q, longest), expect(p, [rows], [n - rows], q), f"longest {longest}")
     p.close()
+
+
+@FORMATS
+@pytest.mark.parametrize("n", [1, 200])
+def test_queries_that_are_not_finite(kxlib, n, f32):
+    """The scores of such a query are infinite or not numbers, whatever the sign, and so is the softmax of them; the other heads and rows are as they would be."""
+    for rows in (1, 5, 80):
+        if rows > n:
+            continue
+        say(f"not finite, {rows} of {n} rows, f32={f32}")
+        p = S.Paged(kxlib, heads=4, kv=2, dim=64, vdim=64, block=16, f32=f32, tokens=n + 2, pages=8)
+        k = np.random.default_rng(6).uniform(1, 2, (n, 2, 64)).astype(np.float32)
+        p.append([n], [0], k=k, v=k[::-1].copy())
+        q = p.queries(rows, 0.5)
+        want = expect(p, [rows], [n - rows], q)
+        bad = np.zeros((rows, 4), bool)
+        for i, x in enumerate((-np.inf, np.inf, np.nan)):
+            row, head = (i * 2) % rows, i
+            q[row, 2 + head * 64 + 9 * i] = x
+            bad[row, head] = True
+        got = attend(p, [rows], [n - rows], q)
+        assert np.isnan(got[bad]).all()
+        near(got[~bad], (want[0][~bad], want[1][~bad]))
+        p.close()
