@@ -1,8 +1,9 @@
 // kx_arrive.h -- "the last one in finishes the job": how workgroups of one launch hand results to each other
 // without anybody waiting.  Used by the q_b GEMV that completes a head's query (kx_dense.hip), the router GEMV
 // whose last workgroup does top-k and bucketing (kx_dense.hip), the routed down GEMV that combines a block
-// of rows (kx_i4.hip) and the products that split a tile's columns (kx_gemm_tile.h in kx_linear.hip and kx_dense_gemm.hip,
-// lin_narrow_k in kx_linear.hip).  No counterpart in the reference, which runs each of these steps as a launch of its own
+// of rows (kx_i4.hip), the products that split a tile's columns (kx_gemm_tile.h in kx_linear.hip, kx_dense_gemm.hip and
+// kx_fp8.hip, lin_narrow_k in kx_linear.hip, fp8_narrow_k in kx_fp8.hip) and the attention that splits positions
+// (kx_paged_attend.hip).  No counterpart in the reference, which runs each of these steps as a launch of its own
 // (src/kimi_exec.cu:812-877).
 //
 // Protocol.  Every group (a workgroup on the GPU, a thread in the host model of it) first writes its results,
@@ -42,7 +43,7 @@
 // The plain accesses on these paths (routing weights, the residual row that is read, modified and written, the
 // counter reset) touch only data that an earlier launch wrote or that no other workgroup of this launch touches.
 // The GPU tests hold the kernels of kx_dense.hip and kx_i4.hip to the oracle's bits in both forms of launch (fused and
-// separate), which would differ if a finisher ever read a stale value; the split products, which are held to a tolerance, have to
+// separate), which would differ if a finisher ever read a stale value; the split products and attentions, which are held to a tolerance, have to
 // give the same bits again and again.  All of them are compared to the bit with the library compiled in form (1).
 //
 // The same header compiles for the host (tests build a thread model of the protocol under ThreadSanitizer: in

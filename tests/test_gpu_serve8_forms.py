@@ -1,0 +1,72 @@
+"""Forms of the 8-bit serving operators that a call takes by sizes and strides alone: results whose rows are whole pieces, and parts that the last workgroup in adds up, in both forms of the hand-over."""
+import os
+
+import numpy as np
+import pytest
+
+import serve8 as S
+from blok_amd.lib import check, load_library
+from kxt import say
+from test_gpu_fp8 import handle, rows_of
+from test_gpu_fp8 import near as product_near
+from test_gpu_serve8_weights import attend, expect, near
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+
+
+@pytest.fixture(scope="module")
+def strict(pytestconfig):
+    """The library whose workgroups hand over in the form of the memory model."""
+    return load_library(os.path.join(str(pytestconfig.rootpath), "blok_amd", "libkx_strict.so"))
+
+
+@FORMATS
+@pytest.mark.parametrize("dim,vdim", [(64, 64), (80, 80), (96, 96), (128, 128), (192, 128), (256, 256), (64, 60)])
+def test_results_in_whole_pieces(kxlib, dim, vdim, f32):
+    """Rows of results that begin at multiples of four elements and rows that do not hold the same bits, from one part and from several; nothing beside them is written."""
+    say(f"pieces of {dim} / {vdim} f32={f32}")
+    lens = [700, 1, 65]
+    p = S.Paged(kxlib, heads=6, kv=2, dim=dim, vdim=vdim, rot=dim // 2, block=64, batch=3, f32=f32, tokens=1000, pages=20)
+    p.append(lens, [0] * 3)
+    for new in ([1, 1, 1], [6, 0, 9], [60, 1, 30]):
+        pos, q = [n - m for n, m in zip(lens, new)], p.queries(sum(new))
+        want = expect(p, new, pos, q)
+        for longest in (1, 700):
+            held = [attend(p, new, pos, q, longest, pad=pad) for pad in (0, 4, 3)]
+            near(held[0], want, f"{new} longest {longest}")
+            for other in held[1:]:
+                np.testing.assert_array_equal(other, held[0])
+    p.close()
+
+
+@FORMATS
+@pytest.mark.parametrize("heads,kv,new", [(8, 1, [1, 1]), (8, 1, [5, 5]), (4, 2, [39, 35])], ids=str)
+def test_parts_of_an_attention_in_both_forms_of_handing_over(kxlib, strict, heads, kv, new, f32):
+    """Few columns, several blocks of them, and columns that waves have for themselves: the same bits again and again."""
+    say(f"attention of {new} rows, {heads} heads, f32={f32}")
+    lens = [4000, 900]
+    p = S.Paged(kxlib, heads=heads, kv=kv, dim=128, vdim=128, block=64, batch=2, f32=f32, tokens=5000, pages=80)
+    p.append(lens, [0, 0])
+    pos, q = [n - m for n, m in zip(lens, new)], p.queries(sum(new))
+    first = attend(p, new, pos, q)
+    near(first, expect(p, new, pos, q))
+    for lib in (None, strict, None, strict, strict):
+        np.testing.assert_array_equal(attend(p, new, pos, q, lib=lib), first)
+    p.close()
+
+
+@pytest.mark.parametrize("out_f32", [False, True])
+@pytest.mark.parametrize("tokens,rows,cols", [(40, 24, 33000), (20, 130, 24000), (64, 70, 9000), (70, 300, 9000), (333, 300, 4000)])
+def test_parts_of_a_product_in_both_forms_of_handing_over(kxlib, strict, tokens, rows, cols, out_f32):
+    """Parts of the columns, of up to 64 tokens and of tiles: the same bits again and again."""
+    say(f"product {tokens} x {rows} x {cols} out_f32={out_f32}")
+    rng = np.random.default_rng(tokens)
+    c, s, w = S.matrix(rng, rows, cols)
+    h, x = handle(kxlib, tokens, cols), rows_of(rng, tokens, cols, False)
+    first = S.product(kxlib, h, c, s, x, cols, out_f32, False)
+    product_near(first, S.row_codes(x), w, out_f32)
+    for lib in (kxlib, strict, kxlib, strict, strict):
+        np.testing.assert_array_equal(S.product(lib, h, c, s, x, cols, out_f32, False), first)
+    check(kxlib.kx_fp8_destroy(h))
