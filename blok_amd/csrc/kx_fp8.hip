@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(N::THREADS, 2) fp8_narrow_k(KxFp8Args a, int p
 bool read_once(const KxFp8Args &a) { return (size_t)a.rows * a.ld >= kxonce::MATRIX; }
 bool in_pieces(const KxFp8Args &a) { return (uintptr_t)a.x % 16 == 0 && (size_t)a.x_ld * (a.x_f32 ? 4 : 2) % 16 == 0; }
 
+constexpr int LDS = 160 * 1024;  // of a CU
 template <class K>
 int allow_lds(K kernel, int bytes, std::atomic<bool> &done) {  // setting it twice from two threads is harmless
   if (!done) {
@@ -377,12 +378,17 @@ int allow_lds(K kernel, int bytes, std::atomic<bool> &done) {  // setting it twi
   }
   return KX_OK;
 }
+// bytes of LDS with the scales of a share's rows, which matrices of millions of rows have too many of
+template <class N>
+int stream_lds(const KxFp8Args &a, int grid) {
+  const int share = kx_cdiv(kx_cdiv(a.rows, 4), grid) * 4;
+  return N::lds(a, (share + 126) / 128 + 1);
+}
 template <class N, bool F32, bool X32, bool ONCE>
 int launch_stream(const KxFp8Args &a, int grid, hipStream_t st) {
   static std::atomic<bool> attr{false};
-  KX_DO(allow_lds(fp8_stream_k<N, F32, X32, ONCE>, 160 * 1024, attr));
-  const int share = kx_cdiv(kx_cdiv(a.rows, 4), grid) * 4, bands = (share + 126) / 128 + 1;
-  fp8_stream_k<N, F32, X32, ONCE><<<(unsigned)grid, N::THREADS, N::lds(a, bands), st>>>(a, in_pieces(a), (N::x_bytes(a) + 15) & ~15);
+  KX_DO(allow_lds(fp8_stream_k<N, F32, X32, ONCE>, LDS, attr));
+  fp8_stream_k<N, F32, X32, ONCE><<<(unsigned)grid, N::THREADS, stream_lds<N>(a, grid), st>>>(a, in_pieces(a), (N::x_bytes(a) + 15) & ~15);
   KX_LAUNCH_CHECK();
   return KX_OK;
 }
@@ -504,12 +510,12 @@ int tiles(const KxFp8Args &a, hipStream_t st) {
 // The tiles of 64 tokens take over where they are as soon: 128 x 7168 x 8192 29.7, 64 of fp8_narrow_k 29.9, 32 of it 23.9.
 int kx_fp8_launch(const KxFp8Args &a, hipStream_t st) {
   const int cus = std::max(1, kx_device_cus()), stream = std::min(kx_cdiv(a.rows, 16), cus);
-  if (a.tokens <= 4 && a.tokens * a.blocks <= 256) return launch_stream<Stream<0, 1, 8, 4>>(a, stream, st);
+  if (a.tokens <= 4 && a.tokens * a.blocks <= 256 && stream_lds<Stream<0, 1, 8, 4>>(a, stream) <= LDS) return launch_stream<Stream<0, 1, 8, 4>>(a, stream, st);
   const dim3 rows(kx_cdiv(a.blocks, 16), std::min(a.tokens, 65535));
   if (a.x_f32) fp8_rows_k<true><<<rows, 256, 0, st>>>(a, in_pieces(a));
   else fp8_rows_k<false><<<rows, 256, 0, st>>>(a, in_pieces(a));
   KX_LAUNCH_CHECK();
-  if (a.tokens <= 32 && a.blocks <= 160) {  // their exponents fit
+  if (a.tokens <= 32 && a.blocks <= 160 && std::max(stream_lds<Stream<2, 1, 8, 2>>(a, stream), stream_lds<Stream<1, 2, 8, 2>>(a, cus)) <= LDS) {
     if (a.tokens > 16) return launch_stream<Stream<2, 1, 8, 2>>(a, stream, st);
     if (a.rows < 64 * cus) return launch_stream<Stream<1, 1, 8, 3>>(a, stream, st);
     return launch_stream<Stream<1, 2, 8, 2>>(a, cus, st);
@@ -572,6 +578,7 @@ extern "C" int kx_fp8_destroy(kx_fp8 *p) {
 extern "C" int kx_fp8_run(kx_fp8 *p, const kx_fp8_args *x, void *stream) {
   KX_REQUIRE(p && x && x->d_w && x->d_w_scale && x->d_x && x->d_out, "kx_fp8_run: null argument");
   KX_REQUIRE(x->tokens >= 0 && x->tokens <= p->max_tokens && x->rows > 0 && x->cols > 0 && x->cols <= p->max_blocks * 128, "kx_fp8_run: tokens=%d rows=%d cols=%d", x->tokens, x->rows, x->cols);
+  KX_REQUIRE(x->rows <= 1 << 25, "kx_fp8_run: rows=%d", x->rows);  // shares of rows are worked out in 32 bits (kxtile::cut)
   KxFp8Args a = p->a;
   a.blocks = kx_cdiv(x->cols, 128);
   KX_REQUIRE(x->ld % 128 == 0 && x->ld >= a.blocks * 128 && x->ld < 1 << 24 && x->x_ld >= x->cols && x->out_ld >= x->rows, "kx_fp8_run: ld=%d x_ld=%d out_ld=%d", x->ld, x->x_ld, x->out_ld);

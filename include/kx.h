@@ -439,7 +439,7 @@ int kx_paged_attend(kx_paged *p, const kx_paged_cache *cache, const kx_paged_row
 int kx_paged_read(kx_paged *p, const kx_paged_cache *cache, const kx_paged_rows *rows, void *d_k, int32_t k_ld, void *d_v, int32_t v_ld, void *stream);
 int kx_paged_faults(kx_paged *p, int32_t *h_bits, void *stream);
 /* ---- products with 8-bit matrices ----------------------------------------------------------
- * kx_fp8_run: y = W x for matrices of e4m3 elements with a scale for each block of 128 x 128, as block-scaled checkpoints have them: d_w [rows][ld], ld a
+ * kx_fp8_run: y = W x for matrices of e4m3 elements with a scale for each block of 128 x 128, as block-scaled checkpoints have them: d_w [rows][ld], at most 2^25 rows, ld a
  * multiple of 128, zero beyond cols; d_w_scale f32 [ceil(rows / 128)][ceil(cols / 128)]; element = code * scale.  A row of x (d_x [tokens][x_ld], float or
  * bf16) is rounded to e4m3 with a scale 2^e for each 128 columns, the least e >= -100 that keeps their largest finite magnitude within
  * 448 * 2^e; what is not finite becomes NaN.  Products and sums are 32-bit; d_out [tokens][out_ld] is float or bf16.  d_w begins at a multiple of 16

@@ -1,11 +1,12 @@
 """Forms of the 8-bit serving operators that a call takes by sizes and strides alone: results whose rows are whole pieces, and parts that the last workgroup in adds up, in both forms of the hand-over."""
+import ctypes as C
 import os
 
 import numpy as np
 import pytest
 
 import serve8 as S
-from blok_amd.lib import check, load_library
+from blok_amd.lib import DevBuf, KxFp8Args, check, load_library
 from kxt import say
 from test_gpu_fp8 import handle, rows_of
 from test_gpu_fp8 import near as product_near
@@ -69,4 +70,39 @@ def test_parts_of_a_product_in_both_forms_of_handing_over(kxlib, strict, tokens,
     product_near(first, S.row_codes(x), w, out_f32)
     for lib in (kxlib, strict, kxlib, strict, strict):
         np.testing.assert_array_equal(S.product(lib, h, c, s, x, cols, out_f32, False), first)
+    check(kxlib.kx_fp8_destroy(h))
+
+
+def test_products_of_too_many_rows_are_refused(kxlib):
+    """Shares of the rows are worked out in 32 bits, which 2^26 rows and 256 workgroups pass."""
+    say("too many rows")
+    h, d = handle(kxlib, 4, 128), DevBuf(1 << 20)
+    for rows in ((1 << 25) + 1, 1 << 26, 2 ** 31 - 1):
+        for tokens in (0, 1, 4):
+            a = KxFp8Args(x_f32=0, out_f32=0, tokens=tokens, rows=rows, cols=128, ld=128, x_ld=128, out_ld=rows, d_w=d.ptr, d_w_scale=d.ptr, d_x=d.ptr, d_out=d.ptr)
+            assert kxlib.kx_fp8_run(h, C.byref(a), None) != 0 and b"kx_fp8_run: rows" in kxlib.kx_last_error()
+    check(kxlib.kx_fp8_destroy(h))
+
+
+def test_products_whose_scales_do_not_fit_beside_a_share(kxlib):
+    """As many rows as there may be: the scales of a workgroup's rows are more than its LDS holds, so that the product is worked out in blocks of rows.  Some rows are looked at."""
+    say("scales beside a share")
+    tokens, rows, cols, ld = 5, 1 << 25, 1100, 1152
+    rng = np.random.default_rng(12)
+    d, at = DevBuf(rows * ld), [0, 1 << 24, rows - 128]              # 39 GB, of which these three bands of 128 rows are set
+    scales = np.full((rows // 128, 9), np.nan, np.float32)
+    w = []
+    for a in at:
+        c, s, x = S.matrix(rng, 128, cols)
+        check(kxlib.kx_h2d(d.ptr + a * ld, c.ctypes.data, c.nbytes))
+        scales[a // 128] = s
+        w.append(x)
+    x, ds = rows_of(rng, tokens, cols, True), DevBuf.from_numpy(scales)
+    dx, out, h = DevBuf.from_numpy(x), DevBuf(tokens * rows * 4), handle(kxlib, tokens, cols)
+    a = KxFp8Args(x_f32=1, out_f32=1, tokens=tokens, rows=rows, cols=cols, ld=ld, x_ld=cols, out_ld=rows, d_w=d.ptr, d_w_scale=ds.ptr, d_x=dx.ptr, d_out=out.ptr)
+    check(kxlib.kx_fp8_run(h, C.byref(a), None))
+    check(kxlib.kx_sync(None))
+    for first, m in zip(at, w):
+        got = np.stack([out.to_numpy(np.float32, (128,), (t * rows + first) * 4) for t in range(tokens)])
+        product_near(got.astype(np.float64), S.row_codes(x), m, True)
     check(kxlib.kx_fp8_destroy(h))
