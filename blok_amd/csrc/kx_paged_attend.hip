@@ -78,6 +78,13 @@ __device__ __forceinline__ float quarters_max(float v) {
   kxw::swap_rows16(v, o);
   return fmaxf(v, o);
 }
+__device__ __forceinline__ uint32_t quarters_max(uint32_t v) {
+  float f = kx_bits_f32(v), o = f;
+  kxw::swap_halves32(f, o);
+  f = o = kx_bits_f32(max(kx_f32_bits(f), kx_f32_bits(o)));
+  kxw::swap_rows16(f, o);
+  return max(kx_f32_bits(f), kx_f32_bits(o));
+}
 __device__ __forceinline__ float quarters_sum(float v) {
   float o = v;
   kxw::swap_halves32(v, o);
@@ -252,21 +259,16 @@ __global__ void __launch_bounds__(FM::THREADS, FM::WAVES) attend_k(KxPagedArgs a
     __syncthreads();
 #pragma unroll
     for (int n = n0; n < (SHARE ? NQ : n0 + 1); ++n) {
-      float most = 0.0f;
-      bool finite = true;
+      uint32_t most = 0;  // bits of the largest magnitude; those of what is not finite are above those of all that is
       const float *const mine = rows + ((n - n0) * 16 + lc) * FM::QLD + lq * 16;
 #pragma unroll
       for (int j = 0; j < DP / 64; ++j)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = __builtin_fabsf(mine[j * 64 + e]);
-          finite &= x < __builtin_inff();
-          most = fmaxf(most, x < __builtin_inff() ? x : 0.0f);
-        }
+        for (int e = 0; e < 16; ++e) most = max(most, kx_f32_bits(mine[j * 64 + e]) & 0x7fffffffu);
       most = quarters_max(most);
-      const int e = max((int)(kx_f32_bits(most) >> 23) - 141, -100);  // the largest element becomes 2^14 or more: f16 has 2^-24 beside it
-      // a query that is not finite has infinite scores or none, and NaN for their softmax: NaN in any element, where minus infinity would hide its positions
-      const float down = !finite ? __builtin_nanf("") : s.scale == 0.0f ? 0.0f : __builtin_copysignf(kx_bits_f32(scale_bits(-e)), s.scale);
+      const int e = max((int)(most >> 23) - 141, -100);  // the largest element becomes 2^14 or more: f16 has 2^-24 beside it
+      // a query that is not finite has infinite scores or none, and NaN for their softmax: NaN in all elements, where minus infinity would hide its positions
+      const float down = most >= 0x7f800000u ? __builtin_nanf("") : s.scale == 0.0f ? 0.0f : __builtin_copysignf(kx_bits_f32(scale_bits(-e)), s.scale);
       qf[n] = kx_bits_f32(scale_bits(e)) * __builtin_fabsf(s.scale) * 1.44269504088896341f;
 #pragma unroll
       for (int j = 0; j < DP / 64; ++j)
