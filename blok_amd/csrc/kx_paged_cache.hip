@@ -440,6 +440,9 @@ extern "C" int kx_paged_attend(kx_paged *p, const kx_paged_cache *cache, const k
 }
 extern "C" int kx_paged_faults(kx_paged *p, int32_t *h_bits, void *stream) {
   KX_REQUIRE(p && h_bits, "kx_paged_faults: null argument");
+  int dev = -1;
+  KX_HIP(hipGetDevice(&dev));
+  KX_REQUIRE(dev == p->device, "kx_paged_faults: made on device %d, called on device %d", p->device, dev);
   KX_HIP(hipStreamSynchronize(kx_stream(stream)));
   KX_HIP(hipMemcpy(h_bits, p->a.fault, 4, hipMemcpyDeviceToHost));
   if (*h_bits) {
