@@ -477,9 +477,9 @@ int launch_tiles(const KxFp8Args &a, kxtile::Share share, hipStream_t st) {
   return KX_OK;
 }
 // The tile that is sooner by estimates in us, and how it is shared out: rounds of one workgroup per CU, and for parts of the columns what handing over their sums takes.
-// us, tiles of 256 / 128 / 64 tokens: 2048 x 18432 x 7168 323 / 346 / 523, 2048 x 7168 x 8192 143 / 166 / 246, 2048 x 2112 x 7168 89 / 86 / 89, 1024 x 12288 x 1536 42 / 47 /
-// 51, 512 x 7168 x 8192 80 / 58 / 59, 256 x 7168 x 2048 53 / 34 / 22, 128 x 18432 x 7168 77 / 56 / 61, 128 x 7168 x 8192 94 / 47 / 30, 96 x 2112 x 7168 81 / 42 / 25; 32-bit
-// results 2048 x 7168 x 8192 - / 288 / 349, 333 x 4103 x 2000 - / 37 / 31.
+// us with the rows before it, tiles of 256 / 128 / 64 tokens: 2048 x 18432 x 7168 296 / 323 / 514, 2048 x 7168 x 8192 128 / 153 / 237, 2048 x 2112 x 7168 80 / 74 / 79 (the
+// estimate takes the first), 1024 x 12288 x 1536 41 / 46 / 49, 512 x 7168 x 8192 79 / 54 / 57, 256 x 7168 x 2048 43 / 28 / 22, 128 x 18432 x 7168 77 / 56 / 63, 128 x 7168 x 8192 69 /
+// 42 / 30, 96 x 2112 x 7168 65 / 38 / 26; 32-bit results 2048 x 7168 x 8192 - / 280 / 339, 333 x 4103 x 2000 - / 36 / 27.
 template <bool F32>
 int tiles(const KxFp8Args &a, hipStream_t st) {
   const int cus = std::max(1, kx_device_cus());

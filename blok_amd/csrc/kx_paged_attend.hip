@@ -15,8 +15,9 @@
 // Two forms: few columns a sequence (SHARE): the waves of a workgroup take groups of tokens in turn and are added up in LDS; many: every wave has columns
 // of its own.  In both the positions may be split between workgroups, and the last one in adds the parts (kx_arrive.h), in order.
 // What bounds it: few columns, HBM -- one position after 131072, 269 MB, 52 us, 11 of them the start and the parts; 64 sequences of up to 8192, 640 MB, 124 us, whose
-// lengths differ -- and for short caches the chain from the tables to the pages and the hand-over, 11 us after 4096.  Many columns, vector instructions beside the
-// matrix cores (128 conversions of codes and 32 exponentials for 64 products of a wave): 590 TFLOP/s of 1200.
+// lengths differ -- and for short caches the chain from the tables to the pages and the hand-over, 11 us after 4096.  Many columns: vector instructions (128 conversions
+// of codes and 32 exponentials for 64 products of a wave), which a SIMD issues in 55 % of the cycles, with its matrix core busy in 24 % and 1.6 waves on average: 580
+// TFLOP/s of 1200.
 #include <algorithm>
 #include <type_traits>
 #include "kx_arrive.h"
@@ -656,12 +657,12 @@ int launch(KxPagedArgs a, int g, hipStream_t st) {
   const int units = (int)((std::max<long>(most, 1) + UNIT - 1) / UNIT);
   const long busy = (long)std::min(a.batch, a.tokens) * ((rows * g + FM::COLS - 1) / FM::COLS) * kv;  // workgroups of whole sequences
   const long room = std::min<long>({(long)(a.part_floats / FM::PART) / std::max<long>(1, tasks * kv), STATS / FM::COLS, units});
-  // a workgroup for each that the card holds; one a CU where a few long sequences fill it evenly: 1 x 131072 55.9 -> 52.5 us, 2 x 131072 88.4 -> 84.8, but 16 x 8192
-  // 41.7 -> 42.9 and 40 x 8192 95 -> 126, whose sequences differ in length
+  // a workgroup for each that the card holds; one a CU where a few long sequences fill it evenly: 1 x 131072 56.0 -> 51.9 us, 2 x 131072 87.3 -> 82.7, but 16 x 8192
+  // 41.5 -> 42.4 and 40 x 8192 94 -> 126, whose sequences differ in length
   const long slots = (long)cus * (FM::ONCE && busy * 8 <= cus ? 1 : FM::WAVES), want = (slots + busy - 1) / busy;
   // Where waves share columns, a part has a group for each at least, and where more than 256 columns of parts are for one workgroup to add up, eight.  Where
-  // they do not, adding up 128 columns takes as long as 12 groups, and a part has 20: 256 rows after 7744, 6 parts 245 -> 126 us, 100 rows after 7900 231 -> 86,
-  // but 300 rows after 1700 in 2 parts 69 -> 77, 100 rows after 500 31 -> 37.
+  // they do not, adding up 128 columns takes as long as 12 groups, and a part has 20: 256 rows after 7744, 6 parts 251 -> 129 us, 100 rows after 7900 237 -> 89,
+  // but 300 rows after 1700 in 2 parts 72 -> 79, 100 rows after 500 32 -> 38.
   const long most_parts = FM::SHARE ? std::max<long>(std::min<long>(units / FM::NW, 256 / FM::COLS), units / (FM::NW * 8)) : units / 20;
   a.splits = (int)std::max<long>(1, std::min({room, want, most_parts}));
   a.chunk = (units + a.splits - 1) / a.splits;
@@ -677,8 +678,8 @@ int launch_columns(const KxPagedArgs &a, hipStream_t st) {
   const int g = a.s.heads / a.s.kv_heads;
   const long columns = (long)a.tokens * g / std::min(a.batch, a.tokens);  // of a sequence, on average
   constexpr int NQ = DP == 256 ? 1 : 2;  // the widest rows leave registers for one block of columns
-  // a cache that no level of caches holds is read past them where one workgroup reads each of its positions: 269 MB 62 -> 56 us, 640 MB 128 -> 124; with 131 MB,
-  // which the last level holds from one call to the next in a program of one layer, it takes 27 us instead of 24
+  // a cache that no level of caches holds is read past them where one workgroup reads each of its positions: 269 MB 61.8 -> 51.9 us with fewer parts, 56.0 with as
+  // many, 640 MB 127 -> 124; with 131 MB, which the last level holds from one call to the next in a program of one layer, it takes 33.3 us instead of 31.3
   const size_t seen = a.s.size ? std::min(a.longest, a.s.size) : a.longest;
   if (columns <= 16 && kxonce::latent((size_t)std::min(a.batch, a.tokens) * seen * a.s.kv_heads * (DP + VP))) return launch<Form<DP, VP, 1, true, F32, true>>(a, g, st);
   if (columns <= 16) return launch<Form<DP, VP, 1, true, F32>>(a, g, st);

@@ -442,7 +442,10 @@ int kx_paged_faults(kx_paged *p, int32_t *h_bits, void *stream);
  * kx_fp8_run: y = W x for matrices of e4m3 elements with a scale for each block of 128 x 128, as block-scaled checkpoints have them: d_w [rows][ld], at most 2^25 rows, ld a
  * multiple of 128, zero beyond cols; d_w_scale f32 [ceil(rows / 128)][ceil(cols / 128)]; element = code * scale.  A row of x (d_x [tokens][x_ld], float or
  * bf16) is rounded to e4m3 with a scale 2^e for each 128 columns, the least e >= -100 that keeps their largest finite magnitude within
- * 448 * 2^e; what is not finite becomes NaN.  Products and sums are 32-bit; d_out [tokens][out_ld] is float or bf16.  d_w begins at a multiple of 16
+ * 448 * 2^e; what is not finite becomes NaN.  d_out [tokens][out_ld] is float or bf16.  For float results
+ * products and sums are 32-bit; for bf16 results the matrix cores add the products of 128 columns in fewer bits, 1.4e-5 off on average and less than 2^-14 of the sum of
+ * their magnitudes in all tests; blocks are scaled and added in 32 bits, and a block's sum is a float without the matrix's scale, which |x| of 2^111 and more may
+ * pass.  d_w begins at a multiple of 16
  * bytes.  No counterpart in the reference.  kx_fp8_create: scratch for rows of up to max_cols columns (at most 131072), max_tokens of them, on the current device;
  * calls on one handle that overlap race. */
 typedef struct kx_fp8_args {
