@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import serve8 as S
-from blok_amd.lib import DevBuf, KxFp8Args, check, load_library
+from blok_amd.lib import DevBuf, KxFp8Args, KxPagedConfig, check, load_library
 from kxt import say
 from test_gpu_fp8 import handle, rows_of
 from test_gpu_fp8 import near as product_near
@@ -106,3 +106,28 @@ def test_products_whose_scales_do_not_fit_beside_a_share(kxlib):
         got = np.stack([out.to_numpy(np.float32, (128,), (t * rows + first) * 4) for t in range(tokens)])
         product_near(got.astype(np.float64), S.row_codes(x), m, True)
     check(kxlib.kx_fp8_destroy(h))
+
+
+@FORMATS
+def test_caches_of_more_than_four_gigabytes(kxlib, f32):
+    """Pages whose places, and places of scales, pass 32 bits; what the memory held before is of no account."""
+    say(f"large cache f32={f32}")
+    pages, page, kv, dim = 36, 1 << 20, 2, 64
+    p = S.Paged(kxlib, heads=4, kv=kv, dim=dim, vdim=dim, rot=dim, block=16, batch=3, f32=f32, tokens=800)
+    check(kxlib.kx_paged_destroy(p.h))
+    p.page, p.pages, p.h = page, pages, C.c_void_p()
+    cfg = KxPagedConfig(4, kv, dim, dim, page, 16, dim, 0, 0, p.scale, 10000.0)
+    check(kxlib.kx_paged_create(C.byref(cfg), None, int(f32), 3, 800, C.byref(p.h)))
+    p.dk, p.dv = DevBuf(pages * kv * page * dim), DevBuf(pages * kv * page * dim)      # 4.8 GB each
+    p.dks, p.dvs = DevBuf(pages * kv * page // 16 * 4), DevBuf(pages * kv * page // 16 * 4)
+    p.free = [0, 17, pages - 1]
+    lens = [300, 65, 120]
+    p.append(lens, [0] * 3)
+    for b, (k, v) in enumerate(p.read(lens, [0] * 3)):
+        np.testing.assert_array_equal(k, p.k[b])
+        np.testing.assert_array_equal(v, p.v[b])
+    for new in ([1, 1, 1], [70, 3, 90]):
+        pos, q = [n - m for n, m in zip(lens, new)], p.queries(sum(new))
+        near(attend(p, new, pos, q), expect(p, new, pos, q))
+    assert p.faults() == 0
+    p.close()

@@ -159,3 +159,25 @@ def test_queries_that_are_not_finite(kxlib, n, f32):
         assert np.isnan(got[bad]).all()
         near(got[~bad], (want[0][~bad], want[1][~bad]))
         p.close()
+
+
+@FORMATS
+@pytest.mark.parametrize("rows,heads", ROWS)
+def test_values_far_below_the_largest_of_their_block(kxlib, rows, heads, f32):
+    """The largest value of each block is one that no row has a weight for, and all others are codes from 2^-9, the smallest there is, to 2^-4: subnormal numbers of every format that they go through."""
+    say(f"{rows} rows of {heads} heads, small codes, f32={f32}")
+    n = 700
+    p = S.Paged(kxlib, heads=heads, kv=1, dim=64, vdim=64, block=16, f32=f32, tokens=n, pages=12)
+    r = np.random.default_rng(11)
+    k, v = (0.1 * r.standard_normal((n, 1, 64))).astype(np.float32), np.ldexp(1.0, r.integers(-9, -3, (n, 1, 64))).astype(np.float32)
+    k[:, 0, 0] = 16.0
+    k[::16], v[::16] = 0.0, 448.0
+    p.append([n], [0], k=k, v=v)
+    assert (p.v[0][1:16] == v[1:16]).all()
+    q = p.queries(rows, 0.5)
+    q[:, 2:2 + heads * 64:64] = 120 * np.log(2.0) / (16 * p.scale)      # 2^-120 of the others' weights
+    want = expect(p, [rows], [n - rows], q)
+    assert (want[0] < 0.05).all()
+    for longest in (1, n):
+        near(attend(p, [rows], [n - rows], q, longest), want, f"longest {longest}")
+    p.close()
